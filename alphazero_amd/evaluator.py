@@ -11,7 +11,20 @@ engine for one search step.
 import torch
 
 
-class TorchEvaluator:
+class _Scores:
+    """What an evaluator's network thinks of positions, beside the plain evaluation a search asks for."""
+
+    @torch.no_grad()
+    def score(self, boards, moves=None, top=0):
+        """boards float32 [n, 2, S, S] -> (value [n], policy.Score): the log-probabilities of `moves` ([n] or [n, m]), the
+        entropy and the `top` best alternatives of the network's policy over the legal moves of each position."""
+        from . import policy
+
+        value, logp = self(boards)
+        return value, policy.score(logp, moves, board=boards, top=top)
+
+
+class TorchEvaluator(_Scores):
     """Wraps a torch.nn.Module / ScriptModule returning (value, log_softmax policy)."""
 
     log_priors = True
@@ -55,7 +68,7 @@ class ConstantEvaluator:
         return self._cache[key]
 
 
-class FusedNetEvaluator:
+class FusedNetEvaluator(_Scores):
     """The reference network (src/model.py:9-44, inference mode) evaluated by the
     engine library's own kernel (az_net_eval: f32 matrix-core convolutions with
     the activations resident in LDS) instead of PyTorch.  Takes a module with the

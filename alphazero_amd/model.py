@@ -37,7 +37,21 @@ class PolicyValueNet(nn.Module):
         return cls(shape, conf.CHANNELS, conf.CONV_CHANNELS, conf.FRONT_LAYER_CNT,
                    conf.POLICY_LAYER_CNT, conf.VALUE_LAYER_CNT)
 
-    def forward(self, boards):
+    def heads(self, boards):
+        """(value, policy logits): the answer before its log-softmax."""
         trunk = self.front(boards)
         logits = self.policy(self.policy_conv(trunk)).flatten(1)
-        return self.value(self.value_conv(trunk)), torch.log_softmax(logits, dim=1)
+        return self.value(self.value_conv(trunk)), logits
+
+    def forward(self, boards):
+        value, logits = self.heads(boards)
+        return value, torch.log_softmax(logits, dim=1)
+
+    def loss(self, board, pi, r, mask_illegal=False):
+        """The trainer's loss on records (device tensors, the fields `augment` returns), src/train.py: KL divergence of
+        the policy from pi (batch mean) plus mean squared error of the value.  mask_illegal: the policy is the softmax
+        over the legal moves (the reference trains on all cells)."""
+        from . import policy
+
+        value, logits = self.heads(board)
+        return policy.loss(logits, value, pi, r, board=board if mask_illegal else None)

@@ -431,6 +431,53 @@ int az_net_set_form(int form);
 int az_net_eval(int shape, int n, const float *d_boards, const int *d_leaf_kind, const float *d_params,
                 int front_layers, int policy_layers, int value_layers, float *d_value, float *d_logp, void *stream);
 
+/* ---- operators of a policy row: what a trainer and an analysis front end ask of the network's answer
+ * (src/train.py's KLDivLoss(batchmean) + MSELoss on its samples; src/pbrain-server.py asks for the best move only).
+ * No engine needed; the device current at the call is the one of the pointers and of `stream`.
+ *
+ * A row is `actions` logits (any real numbers: log-probabilities too), d_logits [n][ld] of type `dtype`.  Only the
+ * legal cells of a row count: d_board float32 [n][2][actions] (legal = 0 in both planes) or d_legal bytes
+ * [n][ld_legal] (legal = nonzero; ld_legal 0: one row for all) or neither (every cell); what stands in the other
+ * cells (infinities, NaN) is not looked at.  A row with no legal cell above -inf is EMPTY.  Sums are held in 32 bits
+ * or more and in an order that depends on the sizes only, so the same inputs give the same bits. */
+enum { AZ_F32 = 0, AZ_BF16 = 1, AZ_F16 = 2 };
+enum { AZ_POLICY_MAX_MOVES = 64, AZ_POLICY_MAX_TOP = 32 };
+/* Log-probabilities of m given moves per row (d_moves [n][m], move_bytes 4 or 8), the entropy, and the `top` best
+ * legal moves with their log-probabilities.
+ *   d_logp [n][m]        a negative move (none): 0; an illegal one, or an empty row: -inf; one >= actions: NaN
+ *   d_entropy [n]        (may be NULL) of the distribution over the legal moves; 0 for an empty row
+ *   d_top_moves, d_top_logp [n][top]   best first, equal logits by lowest index; -1 / -inf where no legal cell above -inf is left;
+ *                        NaN cells are never among them
+ *   d_stats [n][2], d_mask [n][az_policy_mask_words]   (may be NULL) what az_policy_score_grad needs
+ * d_work: az_policy_score_work(n, actions, top) bytes (0 up to 1024 actions), used by this call only. */
+long long az_policy_score_work(int n, int actions, int top);
+int az_policy_mask_words(int actions);   /* 0: rows this long keep no mask (the gradient reads board / legal again) */
+int az_policy_score(int n, int actions, const void *d_logits, int dtype, long long ld, const float *d_board,
+                    const unsigned char *d_legal, long long ld_legal, const void *d_moves, int move_bytes, int m, int top,
+                    float *d_logp, float *d_entropy, float *d_top_logp, int *d_top_moves, float *d_stats,
+                    unsigned long long *d_mask, void *d_work, void *stream);
+/* d_dlogits [n][actions] (dense, type of the logits) = gradient for the logits of sum(g_logp * logp) + sum(g_entropy *
+ * entropy); either upstream gradient may be NULL.  Moves that are none, illegal or out of range contribute nothing, a
+ * move given twice twice; masked cells and empty rows get 0.  d_entropy, d_stats, d_mask (may be NULL): as
+ * az_policy_score wrote them. */
+int az_policy_score_grad(int n, int actions, const void *d_logits, int dtype, long long ld, const float *d_board,
+                         const unsigned char *d_legal, long long ld_legal, const unsigned long long *d_mask,
+                         const void *d_moves, int move_bytes, int m, const float *d_g_logp, const float *d_g_entropy,
+                         const float *d_entropy, const float *d_stats, void *d_dlogits, void *stream);
+/* The trainer's loss over n >= 1 records:  1/n sum_i sum_j pi_ij (log pi_ij - log p_ij) + 1/n sum_i (v_i - r_i)^2,
+ * j over the legal cells (targets in masked cells are not looked at, 0 log 0 = 0, an empty row adds its value part only).
+ *   d_value [n]: float32 (value_f32) or the logits' type; d_pi float32 [n][actions]; d_r float32 [n]
+ *   d_loss [3] (may be NULL): total, policy part, value part
+ *   d_dlogits [n][actions] (type of the logits), d_dvalue [n] (type of the values): gradients of the total times
+ *   *d_scale (device float; NULL: 1); either may be NULL.  only_if_scaled: do nothing when *d_scale is 1 (the buffers
+ *   hold the gradients of an earlier call with the same inputs and no scale).
+ * d_work: az_policy_loss_work(n, actions) bytes, used by this call only. */
+long long az_policy_loss_work(int n, int actions);
+int az_policy_loss(int n, int actions, const void *d_logits, int dtype, long long ld, const float *d_board,
+                   const unsigned char *d_legal, long long ld_legal, const void *d_value, int value_f32, const float *d_pi,
+                   const float *d_r, const float *d_scale, int only_if_scaled, float *d_loss, void *d_dlogits,
+                   void *d_dvalue, void *d_work, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
