@@ -1,0 +1,515 @@
+// Newton-Schulz orthogonalisation of weight updates (gfx950): the singular values of G / |G|_F go through
+//   p(s) = a s + b s^3 + c s^5,   (a, b, c) = (3.4445, -4.7750, 2.0315),
+// `steps` times, which moves all but the smallest near 1 and leaves the singular vectors alone.
+//
+// With m <= n (a taller matrix is taken transposed), A = X X' and Q = a I + b A + c A^2, one step is X <- Q X and makes
+// the next Gram matrix A' = Q A Q = Q^2 A: all m x m factors are polynomials of one symmetric matrix, they commute and
+// stay symmetric.  So a group of k steps can be taken on m x m matrices alone and applied to X at once,
+//   A = X X';  Q_1;  A <- (A Q_1) Q_1;  Q_2;  ...;  X <- (Q_k ... Q_1) X,
+// and every m x m product computes its upper tiles only: 3 m^2 n + (4k - 3) m^3 products a group.  What limits k is that a
+// Gram matrix carries an error of 2^-24 |A| into directions whose singular value is near 0, where a step multiplies it
+// by a^2 = 11.9.  Measured error of five steps against 64 bits, next to float32 products (16 x 144, 256 x 256, 256 x
+// 2304):  k = 1  0.9, 0.4, 0.7 times;  k = 2  0.8, 1.2, 1.0;  k = 3  3.2, 11, 0.7.
+//
+// Arithmetic: the matrix cores have no fast float32 product, so a number is held as the sum of two float16 numbers
+// (hi + lo, 22 bits) times a power of two, and a product is hi hi + hi lo + lo hi in float32 accumulators (the missing
+// lo lo is below 2^-22 of the result).  Powers of two put the largest possible entry below float16's limit: entries of
+// X are at most 1.25, of A 1.6, of Q products a^3 = 41.
+//
+// Packed layout of a matrix: rows of K-contiguous groups of 8 numbers, 16 bytes of hi then 16 bytes of lo.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+#include <type_traits>
+
+#include "../../include/azmcts.h"
+
+namespace {
+
+constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
+constexpr int EXP_X = 15, EXP_A = 14, EXP_Q = 10; // stored number = value * 2^EXP
+constexpr int MAX_BATCH = 64;                     // matrices per launch (their addresses travel as kernel arguments)
+constexpr int NORM_PARTS = 64;                    // partial sums of squares per matrix, at most
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+struct bf16_t { uint16_t u; };
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(bf16_t v) { return __uint_as_float((uint32_t)v.u << 16); }
+__device__ __forceinline__ float as_float(_Float16 v) { return (float)v; }
+__device__ __forceinline__ void put(float *p, float v) { *p = v; }
+__device__ __forceinline__ void put(bf16_t *p, float v)
+{
+    const uint32_t b = __float_as_uint(v); // to nearest even; a NaN stays one
+    p->u = v != v ? (uint16_t)0x7fc0 : (uint16_t)((b + 0x7fffu + ((b >> 16) & 1u)) >> 16);
+}
+__device__ __forceinline__ void put(_Float16 *p, float v) { *p = (_Float16)v; }
+
+struct Ptrs { const void *in[MAX_BATCH]; void *out[MAX_BATCH]; };
+
+// the matrices of a launch: G is rows x cols with row pitch ld (elements), X is G or its transpose, m x n with m <= n
+struct Shape {
+    int rows, cols, m, n, mp, np; // mp, np: padded with zeros to whole tiles
+    long long ld_in, ld_out;
+    int tall;
+};
+
+// ---- sum of squares, in 64 bits (a float32 square leaves the range at 1e19 and 1e-23)
+template <class T> __global__ __launch_bounds__(256) void k_norm(Ptrs p, Shape s, int parts, double *sums)
+{
+    const T *g = (const T *)p.in[blockIdx.y];
+    double acc = 0.;
+    for (int i = blockIdx.x * 4 + (threadIdx.x >> 6); i < s.rows; i += parts * 4) {
+        const T *row = g + (size_t)i * s.ld_in;
+        for (int j = threadIdx.x & 63; j < s.cols; j += 64) {
+            const double v = (double)as_float(row[j]);
+            acc = fma(v, v, acc);
+        }
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) acc += __shfl_xor(acc, o);
+    __shared__ double s_w[4];
+    if ((threadIdx.x & 63) == 0) s_w[threadIdx.x >> 6] = acc;
+    __syncthreads();
+    if (threadIdx.x == 0) sums[(size_t)blockIdx.y * NORM_PARTS + blockIdx.x] = (s_w[0] + s_w[1]) + (s_w[2] + s_w[3]);
+}
+
+// hi and lo halves of 8 numbers, 32 bytes at p
+__device__ __forceinline__ void pack8(char *p, const float (&v)[8])
+{
+    h8 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        hi[i] = (_Float16)v[i];
+        lo[i] = (_Float16)(v[i] - (float)hi[i]);
+    }
+    *(h8 *)p = hi;
+    *(h8 *)(p + 16) = lo;
+}
+__device__ __forceinline__ void unpack8(const char *p, float (&v)[8])
+{
+    const h8 hi = *(const h8 *)p, lo = *(const h8 *)(p + 16);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = (float)hi[i] + (float)lo[i];
+}
+
+// G / |G| packed as X [mp][np] and as its transpose [np][mp]; one 64 x 64 tile of G per workgroup
+template <class T> __global__ __launch_bounds__(256) void k_split(Ptrs p, Shape s, int parts, const double *sums, char *X, char *XT)
+{
+    __shared__ float t[64][65];
+    __shared__ double s_scale;
+    const int b = blockIdx.z;
+    const T *g = (const T *)p.in[b];
+    if (threadIdx.x < 64) {
+        double sum = (int)threadIdx.x < parts ? sums[(size_t)b * NORM_PARTS + threadIdx.x] : 0.;
+#pragma unroll
+        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+        if (threadIdx.x == 0) s_scale = sum == 0. ? 0. : ldexp(1. / sqrt(sum), EXP_X);
+    }
+    __syncthreads();
+    const double scale = s_scale;
+    const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+    for (int e = threadIdx.x; e < 64 * 64; e += 256) {
+        const int r = e >> 6, c = e & 63;
+        const bool in = r0 + r < s.rows && c0 + c < s.cols;
+        t[r][c] = in ? (float)((double)as_float(g[(size_t)(r0 + r) * s.ld_in + c0 + c]) * scale) : 0.f;
+    }
+    __syncthreads();
+    // G row-major is X when wide and X' when tall
+    char *same = s.tall ? XT : X, *turned = s.tall ? X : XT;
+    const int rp = s.tall ? s.np : s.mp, cp = s.tall ? s.mp : s.np; // padded rows and columns of G
+    const size_t size = (size_t)s.mp * s.np * 4;
+    for (int e = threadIdx.x; e < 64 * 8; e += 256) {
+        const int r = e >> 3, c = (e & 7) * 8;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = t[r][c + i];
+        if (r0 + r < rp && c0 + c < cp) pack8(same + b * size + ((size_t)(r0 + r) * cp + c0 + c) * 4, v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = t[c + i][r];
+        if (c0 + r < cp && r0 + c < rp) pack8(turned + b * size + ((size_t)(c0 + r) * rp + r0 + c) * 4, v);
+    }
+}
+
+// ---- packed products:  D = alpha * (A B') + beta * E + gamma * I,  A [M][K], B [N][K] packed
+struct Gemm {
+    const char *A, *B;
+    size_t sA, sB;      // bytes from one matrix of the batch to the next
+    int pitchA, pitchB; // bytes per row
+    int K;
+    int tiles_m, tiles_n, symmetric; // symmetric: upper tiles only, each written to both of its places
+    float alpha, beta, gamma;
+    const char *E;      // packed, same shape as D; or NULL
+    size_t sE;
+    char *D, *DT;       // packed result [M][N] and / or its transpose [N][M]; or NULL
+    size_t sD;
+    int pitchD, pitchDT;
+    int user;           // write p.out[] (rows of D are rows of G, or columns when s.tall)
+};
+
+// 16 bytes per lane straight into LDS; the wavefront's 64 lanes fill 1 KB from `lds` on in lane order
+__device__ __forceinline__ void load_lds(const char *g, char *lds)
+{
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)g,
+                                     (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
+}
+
+constexpr int BK = 32;              // K per stage: 128 bytes of a packed row
+// place of 16-byte piece c of row r within the row's 128 bytes: 16 lanes that read the same piece of 16 rows touch
+// all 64 banks
+__device__ __forceinline__ int place(int r, int c) { return c ^ ((r >> 1) & 7); }
+
+// BM x BN results per workgroup of 4 wavefronts (2 x 2); per stage and wavefront (BM/64) (BN/64) 2 x 3 matrix
+// instructions 32x32x16 on (BM/64 + BN/64) 4 LDS reads.  Two stages in LDS: the next one loads while this one is used.
+template <int BM, int BN, class T> __global__ __launch_bounds__(256, 2) void k_gemm(Gemm a, Ptrs p, Shape s)
+{
+    constexpr int FM = BM / 64, FN = BN / 64; // 32 x 32 blocks of a wavefront
+    constexpr int STAGE = (BM + BN) * 128;
+    constexpr int TILE = BM * (BN + 4) * 4;
+    __shared__ __align__(16) char lds[2 * STAGE > TILE ? 2 * STAGE : TILE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = blockIdx.y;
+    // neighbouring tiles share operands: give each of the 8 XCDs (workgroups go round them) a run of tiles
+    int tile;
+    {
+        const int n = gridDim.x, x = blockIdx.x & 7, i = blockIdx.x >> 3, per = n >> 3, rest = n & 7;
+        tile = x * per + min(x, rest) + i;
+    }
+    int ti, tj;
+    if (a.symmetric) {
+        ti = 0;
+        while (tile >= a.tiles_n - ti) tile -= a.tiles_n - ti++;
+        tj = ti + tile;
+    } else {
+        ti = tile / a.tiles_n;
+        tj = tile - ti * a.tiles_n;
+    }
+    const char *A = a.A + b * a.sA + (size_t)ti * BM * a.pitchA;
+    const char *B = a.B + b * a.sB + (size_t)tj * BN * a.pitchB;
+
+    constexpr int LOADS = (BM + BN) / 8 / 4; // 8-row loads per wavefront and stage
+    const char *src[LOADS];
+    int dst[LOADS];
+#pragma unroll
+    for (int l = 0; l < LOADS; l++) {
+        const int r8 = (l * 4 + wave) * 8, r = r8 + (lane >> 3);
+        const int c = place(r, lane & 7);
+        src[l] = r8 < BM ? A + (size_t)r * a.pitchA + c * 16 : B + (size_t)(r - BM) * a.pitchB + c * 16;
+        dst[l] = r8 * 128;
+    }
+    // the small products have accumulators of their own: added to the large ones they would cost a rounding each
+    // (three times the error of one step)
+    f16v acc[FM][FN], low[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[i][j][e] = low[i][j][e] = 0.f;
+    const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
+    const int lr = lane & 31, half = lane >> 5;
+    const int stages = a.K / BK;
+#pragma unroll
+    for (int l = 0; l < LOADS; l++) load_lds(src[l], lds + dst[l]);
+    for (int k = 0; k < stages; k++) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // this wavefront's part of stage k has arrived
+        __syncthreads();                                 // all of it has; nobody reads the other buffer any more
+        const char *cur = lds + (k & 1) * STAGE;
+        if (k + 1 < stages) {
+            char *next = lds + ((k + 1) & 1) * STAGE;
+#pragma unroll
+            for (int l = 0; l < LOADS; l++) load_lds(src[l] + (size_t)(k + 1) * 128, next + dst[l]);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+            h8 ah[FM], al[FM], bh[FN], bl[FN];
+            const int c = (ks * 2 + half) * 2;
+#pragma unroll
+            for (int i = 0; i < FM; i++) {
+                const int r = wm + i * 32 + lr;
+                ah[i] = *(const h8 *)(cur + r * 128 + place(r, c) * 16);
+                al[i] = *(const h8 *)(cur + r * 128 + place(r, c + 1) * 16);
+            }
+#pragma unroll
+            for (int j = 0; j < FN; j++) {
+                const int r = BM + wn + j * 32 + lr;
+                bh[j] = *(const h8 *)(cur + r * 128 + place(r, c) * 16);
+                bl[j] = *(const h8 *)(cur + r * 128 + place(r, c + 1) * 16);
+            }
+#pragma unroll
+            for (int i = 0; i < FM; i++)
+#pragma unroll
+                for (int j = 0; j < FN; j++) {
+                    low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], low[i][j], 0, 0, 0);
+                    low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], low[i][j], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
+                }
+        }
+    }
+    // the tile through LDS, so that every write is a whole group of 8 whichever way the result is stored
+    __syncthreads();
+    float *t = (float *)lds;
+    constexpr int LT = BN + 4;
+#pragma unroll
+    for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int r = wm + i * 32 + (e >> 2) * 8 + half * 4 + (e & 3), c = wn + j * 32 + lr;
+                t[r * LT + c] = (acc[i][j][e] + low[i][j][e]) * a.alpha;
+            }
+    __syncthreads();
+    const int row0 = ti * BM, col0 = tj * BN;
+    if (a.user) {
+        T *out = (T *)p.out[b];
+        for (int e = threadIdx.x; e < BM * BN; e += 256) {
+            if (!s.tall) {
+                const int r = e / BN, c = e % BN;
+                if (row0 + r < s.m && col0 + c < s.n) put(out + (size_t)(row0 + r) * s.ld_out + col0 + c, t[r * LT + c]);
+            } else {
+                const int c = e / BM, r = e % BM;
+                if (row0 + r < s.m && col0 + c < s.n) put(out + (size_t)(col0 + c) * s.ld_out + row0 + r, t[r * LT + c]);
+            }
+        }
+        return;
+    }
+    for (int e = threadIdx.x; e < BM * BN / 8; e += 256) {
+        const int r = e / (BN / 8), c = e % (BN / 8) * 8;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = t[r * LT + c + i];
+        const size_t at = (size_t)(row0 + r) * a.pitchD + (size_t)(col0 + c) * 4;
+        if (a.E) {
+            float w[8];
+            unpack8(a.E + b * a.sE + at, w);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                v[i] = fmaf(a.beta, w[i], v[i]) + (row0 + r == col0 + c + i ? a.gamma : 0.f);
+                t[r * LT + c + i] = v[i];
+            }
+        }
+        if (a.D) pack8(a.D + b * a.sD + at, v);
+    }
+    if (!a.DT || (a.symmetric && ti == tj)) return;
+    __syncthreads();
+    for (int e = threadIdx.x; e < BM * BN / 8; e += 256) {
+        const int c = e / (BM / 8), r = e % (BM / 8) * 8;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = t[(r + i) * LT + c];
+        pack8(a.DT + b * a.sD + (size_t)(col0 + c) * a.pitchDT + (size_t)(row0 + r) * 4, v);
+    }
+}
+
+// ---------------------------------------------------------------- host side
+
+int launch_ok() { return hipGetLastError() == hipSuccess ? AZ_OK : AZ_ERR_HIP; }
+
+template <class F> void by_type(int dtype, F f)
+{
+    if (dtype == AZ_F32) f((float *)nullptr);
+    else if (dtype == AZ_BF16) f((bf16_t *)nullptr);
+    else f((_Float16 *)nullptr);
+}
+
+int round_up(int v, int to) { return (v + to - 1) / to * to; }
+
+Shape shape_of(int rows, int cols)
+{
+    Shape s = {};
+    s.rows = rows;
+    s.cols = cols;
+    s.tall = rows > cols;
+    s.m = s.tall ? cols : rows;
+    s.n = s.tall ? rows : cols;
+    s.mp = round_up(s.m, s.m <= 64 ? 64 : 128);
+    s.np = round_up(s.n, s.n <= 64 ? 64 : 128);
+    return s;
+}
+
+struct Plan {
+    size_t x, mm;     // bytes of a packed X and of a packed m x m matrix
+    size_t sums, total;
+};
+Plan plan_of(const Shape &s, int batch)
+{
+    Plan p;
+    p.x = (size_t)s.mp * s.np * 4;
+    p.mm = (size_t)s.mp * s.mp * 4;
+    p.sums = (size_t)batch * NORM_PARTS * sizeof(double);
+    p.total = p.sums + batch * (3 * p.x + 5 * p.mm);
+    return p;
+}
+
+// launches D = alpha A B' + ... over `batch` matrices
+void gemm(Gemm a, int M, int N, int batch, int dtype, const Ptrs &p, const Shape &s, hipStream_t st)
+{
+    // 128 x 128 tiles halve the operand traffic of 64 x 64 ones, but a launch should have a workgroup for every CU
+    const auto tiles = [&](int t) { return a.symmetric ? (long long)(M / t) * (M / t + 1) / 2 : (long long)(M / t) * (N / t); };
+    const bool big = M % 128 == 0 && N % 128 == 0 && tiles(128) * batch >= 256;
+    const int t = big ? 128 : 64;
+    a.tiles_m = M / t;
+    a.tiles_n = N / t;
+    const dim3 grid((unsigned)tiles(t), batch), block(256);
+    if (!a.user) {
+        if (big) hipLaunchKernelGGL((k_gemm<128, 128, float>), grid, block, 0, st, a, p, s);
+        else hipLaunchKernelGGL((k_gemm<64, 64, float>), grid, block, 0, st, a, p, s);
+        return;
+    }
+    by_type(dtype, [&](auto *d) {
+        using T = std::remove_pointer_t<decltype(d)>;
+        if (big) hipLaunchKernelGGL((k_gemm<128, 128, T>), grid, block, 0, st, a, p, s);
+        else hipLaunchKernelGGL((k_gemm<64, 64, T>), grid, block, 0, st, a, p, s);
+    });
+}
+
+bool shape_ok(int count, int rows, int cols, int dtype, int steps)
+{
+    return count >= 0 && rows >= 1 && cols >= 1 && rows <= AZ_MUON_MAX_DIM && cols <= AZ_MUON_MAX_DIM &&
+           (long long)rows * cols <= AZ_MUON_MAX_CELLS && dtype >= AZ_F32 && dtype <= AZ_F16 && steps >= 1 && steps <= AZ_MUON_MAX_STEPS;
+}
+
+int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *work, hipStream_t st)
+{
+    const Plan pl = plan_of(s, batch);
+    double *sums = (double *)work;
+    char *X = work + pl.sums, *XT = X + batch * pl.x, *YT = XT + batch * pl.x;
+    char *mm[5];
+    for (int i = 0; i < 5; i++) mm[i] = YT + batch * pl.x + i * batch * pl.mm;
+    int parts = (s.rows + 15) / 16;
+    if (parts > NORM_PARTS) parts = NORM_PARTS;
+    const int rp = s.tall ? s.np : s.mp, cp = s.tall ? s.mp : s.np;
+    by_type(dtype, [&](auto *d) {
+        using T = std::remove_pointer_t<decltype(d)>;
+        hipLaunchKernelGGL((k_norm<T>), dim3(parts, batch), dim3(256), 0, st, p, s, parts, sums);
+        hipLaunchKernelGGL((k_split<T>), dim3((cp + 63) / 64, (rp + 63) / 64, batch), dim3(256), 0, st, p, s, parts, (const double *)sums, X, XT);
+    });
+    const auto two = [](int e) { return ldexpf(1.f, e); };
+    const int px = s.np * 4, pm = s.mp * 4;
+    // a symmetric m x m product of two packed ones, 2^ex * 2^ey in the accumulator, stored with 2^eo
+    const auto square = [&](const char *x, int ex, const char *y, int ey, char *out, int eo, float f = 1.f, const char *E = nullptr,
+                            float beta = 0.f, float gamma = 0.f) {
+        Gemm g = {};
+        g.A = x; g.B = y;
+        g.sA = g.sB = g.sE = g.sD = pl.mm;
+        g.pitchA = g.pitchB = g.pitchD = g.pitchDT = pm;
+        g.K = s.mp;
+        g.symmetric = 1;
+        g.alpha = f * two(eo - ex - ey);
+        g.E = E; g.beta = beta; g.gamma = gamma;
+        g.D = g.DT = out;
+        gemm(g, s.mp, s.mp, batch, dtype, p, s, st);
+    };
+    // Steps per group.  Results of 16 bits (half a step: 2^-9, 2^-12) have room for three.  For float32 groups of two
+    // keep the error where single steps have it and pay where X is much wider than high: at n = 4 m they leave 47
+    // of 65 m^3 products, at n = 2 m 29 of 35.
+    const int group = dtype != AZ_F32 ? 3 : s.n >= 4 * s.m ? 2 : 1;
+    for (int left = steps; left > 0;) {
+        // (the odd ones first: the longer groups start from the better conditioned matrix)
+        const int k = left > group ? (left % group ? left % group : group) : left;
+        char *A = mm[0], *T = mm[1], *Q = mm[2], *W = mm[3], *V = mm[4];
+        {
+            Gemm g = {};
+            g.A = g.B = X;
+            g.sA = g.sB = pl.x;
+            g.pitchA = g.pitchB = px;
+            g.K = s.np;
+            g.symmetric = 1;
+            g.alpha = two(EXP_A - 2 * EXP_X);
+            g.sD = pl.mm;
+            g.pitchD = g.pitchDT = pm;
+            g.D = g.DT = A;
+            gemm(g, s.mp, s.mp, batch, dtype, p, s, st);
+        }
+        const auto poly = [&](char *out) { // a I + b A + c A^2
+            square(A, EXP_A, A, EXP_A, out, EXP_Q, NS_C, A, NS_B * two(EXP_Q - EXP_A), NS_A * two(EXP_Q));
+        };
+        poly(W);
+        for (int i = 1; i < k; i++) {
+            // W = the last step's Q; A <- (A W) W, V = the next step's Q, Q = the product of all so far
+            square(A, EXP_A, W, EXP_Q, T, EXP_A);
+            square(T, EXP_A, W, EXP_Q, A, EXP_A);
+            poly(V);
+            square(V, EXP_Q, i == 1 ? W : Q, EXP_Q, T, EXP_Q);
+            char *old = Q;
+            Q = T;
+            T = old;
+            char *w = W;
+            W = V;
+            V = w;
+        }
+        const char *total = k == 1 ? W : Q;
+        left -= k;
+        Gemm g = {};
+        g.A = total; g.B = XT;
+        g.sA = pl.mm; g.sB = pl.x;
+        g.pitchA = g.pitchB = pm;
+        g.K = s.mp;
+        g.user = left == 0;
+        g.alpha = two((left ? EXP_X : 0) - EXP_Q - EXP_X);
+        if (left) { // X is not read here, its transpose is
+            g.sD = pl.x;
+            g.D = X;
+            g.pitchD = px;
+            g.DT = YT;
+            g.pitchDT = pm;
+        }
+        gemm(g, s.mp, s.np, batch, dtype, p, s, st);
+        char *t = XT;
+        XT = YT;
+        YT = t;
+    }
+    return launch_ok();
+}
+
+// Matrices per batch: as many as the kernel arguments hold, but no more than a workspace of 1 GiB needs (matrices that
+// large fill the chip one by one).
+int batch_of(const Shape &s, int count)
+{
+    const size_t one = plan_of(s, 1).total;
+    long long most = (long long)(((size_t)1 << 30) / one);
+    if (most < 1) most = 1;
+    if (most > MAX_BATCH) most = MAX_BATCH;
+    return (int)(count < most ? count : most);
+}
+
+} // namespace
+
+extern "C" {
+
+long long az_muon_work(int count, int rows, int cols)
+{
+    if (!shape_ok(count, rows, cols, AZ_F32, 1)) return -1;
+    if (count == 0) return 0;
+    const Shape s = shape_of(rows, cols);
+    return (long long)plan_of(s, batch_of(s, count)).total;
+}
+
+int az_muon_orthogonalise(int count, int rows, int cols, const void *const *d_in, long long ld_in, void *const *d_out,
+                          long long ld_out, int dtype, int steps, void *d_work, void *stream)
+{
+    if (!shape_ok(count, rows, cols, dtype, steps) || ld_in < cols || ld_out < cols) return AZ_ERR_ARG;
+    if (count == 0) return AZ_OK;
+    if (!d_in || !d_out || !d_work) return AZ_ERR_ARG;
+    for (int i = 0; i < count; i++)
+        if (!d_in[i] || !d_out[i]) return AZ_ERR_ARG;
+    Shape s = shape_of(rows, cols);
+    s.ld_in = ld_in;
+    s.ld_out = ld_out;
+    const int batch = batch_of(s, count);
+    for (int at = 0; at < count; at += batch) {
+        const int n = count - at < batch ? count - at : batch;
+        Ptrs p = {};
+        for (int i = 0; i < n; i++) {
+            p.in[i] = d_in[at + i];
+            p.out[i] = d_out[at + i];
+        }
+        const int rc = run_batch(n, s, dtype, steps, p, (char *)d_work, (hipStream_t)stream);
+        if (rc != AZ_OK) return rc;
+    }
+    return AZ_OK;
+}
+
+} // extern "C"

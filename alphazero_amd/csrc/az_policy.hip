@@ -453,8 +453,8 @@ template <class T, int R> __global__ __launch_bounds__(64 * WAVES) void k_loss(R
     if (o.part) block_part(sum, v, o.part + 2 * (size_t)blockIdx.x);
 }
 
-// loss[0..2] = total, policy, value from the workgroups' partial sums, added in a fixed order
-__global__ __launch_bounds__(64 * WAVES) void k_loss_join(const double *part, int blocks, double inv_n, float *loss)
+// the total, and the policy and value parts, from the workgroups' partial sums, added in a fixed order
+__global__ __launch_bounds__(64 * WAVES) void k_loss_join(const double *part, int blocks, double inv_n, float *loss, float *parts)
 {
     double p = 0., v = 0.;
     for (int i = threadIdx.x; i < blocks; i += 64 * WAVES) {
@@ -465,8 +465,10 @@ __global__ __launch_bounds__(64 * WAVES) void k_loss_join(const double *part, in
     block_part(p, v, s_all);
     if (threadIdx.x == 0) {
         loss[0] = (float)((s_all[0] + s_all[1]) * inv_n);
-        loss[1] = (float)(s_all[0] * inv_n);
-        loss[2] = (float)(s_all[1] * inv_n);
+        if (parts) {
+            parts[0] = (float)(s_all[0] * inv_n);
+            parts[1] = (float)(s_all[1] * inv_n);
+        }
     }
 }
 
@@ -875,12 +877,12 @@ long long az_policy_loss_work(int n, int actions)
 
 int az_policy_loss(int n, int actions, const void *d_logits, int dtype, long long ld, const float *d_board,
                    const unsigned char *d_legal, long long ld_legal, const void *d_value, int value_f32, const float *d_pi,
-                   const float *d_r, const float *d_scale, int only_if_scaled, float *d_loss, void *d_dlogits,
+                   const float *d_r, const float *d_scale, int only_if_scaled, float *d_loss, float *d_parts, void *d_dlogits,
                    void *d_dvalue, void *d_work, void *stream)
 {
     const Rows a = {d_logits, ld, d_board, d_legal, ld_legal, n, actions};
     if (!rows_ok(a, dtype) || n < 1) return AZ_ERR_ARG;
-    if (!d_logits || !d_value || !d_pi || !d_r || !d_work || (only_if_scaled && !d_scale)) return AZ_ERR_ARG;
+    if (!d_logits || !d_value || !d_pi || !d_r || !d_work || (only_if_scaled && !d_scale) || (d_parts && !d_loss)) return AZ_ERR_ARG;
     Loss o = {d_value, value_f32, d_pi, d_r, 1.f / (float)n, d_scale, only_if_scaled, d_loss ? (double *)d_work : nullptr, d_dlogits, d_dvalue};
     const dim3 block(64 * WAVES);
     const hipStream_t st = (hipStream_t)stream;
@@ -908,7 +910,7 @@ int az_policy_loss(int n, int actions, const void *d_logits, int dtype, long lon
             hipLaunchKernelGGL((k_long_loss<T>), dim3(blocks), block, 0, st, a, c, (const Part *)w.part, o);
         });
     }
-    if (d_loss) hipLaunchKernelGGL(k_loss_join, dim3(1), block, 0, st, (const double *)d_work, blocks, 1. / n, d_loss);
+    if (d_loss) hipLaunchKernelGGL(k_loss_join, dim3(1), block, 0, st, (const double *)d_work, blocks, 1. / n, d_loss, d_parts);
     return launch_ok();
 }
 

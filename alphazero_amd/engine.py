@@ -84,7 +84,9 @@ SYMBOLS = [
     ("az_policy_score", _i, [_i, _i, _vp, _i, C.c_longlong, _vp, _vp, C.c_longlong, _vp, _i, _i, _i] + [_vp] * 8),
     ("az_policy_score_grad", _i, [_i, _i, _vp, _i, C.c_longlong, _vp, _vp, C.c_longlong, _vp, _vp, _i, _i] + [_vp] * 6),
     ("az_policy_loss_work", C.c_longlong, [_i, _i]),
-    ("az_policy_loss", _i, [_i, _i, _vp, _i, C.c_longlong, _vp, _vp, C.c_longlong, _vp, _i, _vp, _vp, _vp, _i] + [_vp] * 5),
+    ("az_policy_loss", _i, [_i, _i, _vp, _i, C.c_longlong, _vp, _vp, C.c_longlong, _vp, _i, _vp, _vp, _vp, _i] + [_vp] * 6),
+    ("az_muon_work", C.c_longlong, [_i, _i, _i]),
+    ("az_muon_orthogonalise", _i, [_i, _i, _i, _vp, C.c_longlong, _vp, C.c_longlong, _i, _i, _vp, _vp]),
     ("az_get_prob", _i, [_vp, _i, _vp]),
     ("az_get_board", _i, [_vp, _i, _vp]),
     ("az_get_raw_board", _i, [_vp, _i, _vp]),

@@ -31,14 +31,20 @@ def _ptr(t):
 
 
 def _call(name, device, *args):
-    L = _E.load_library()
+    entry = getattr(_E.load_library(), name)
+    stream = torch._C._cuda_getCurrentRawStream(device.index)  # (torch.cuda.current_stream: 3 us more a call)
     if torch.cuda.current_device() == device.index:
-        rc = getattr(L, name)(*args, torch.cuda.current_stream().cuda_stream)
+        rc = entry(*args, stream)
     else:
         with torch.cuda.device(device):
-            rc = getattr(L, name)(*args, torch.cuda.current_stream().cuda_stream)
+            rc = entry(*args, stream)
     if rc != 0:
         raise RuntimeError(f"{name} failed (code {rc})")
+
+
+def _once():
+    if torch.is_grad_enabled():  # a backward pass that builds a graph of itself
+        raise RuntimeError("the policy operators can be differentiated once (no create_graph)")
 
 
 def _on_one_gpu(**tensors):
@@ -111,8 +117,8 @@ class _ScoreFunction(torch.autograd.Function):
         return logp, entropy, top_moves, top_logp
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_logp, g_entropy, _moves, _logp):
+        _once()
         logits, moves, board, legal, entropy, stats, bits = ctx.saved_tensors
         if g_logp is None and g_entropy is None:
             return None, None, None, None, None
@@ -155,12 +161,12 @@ def score(logits, moves=None, *, board=None, legal=None, top=0):
     return Score(*_score_forward(logits, moves, board, legal, top, False)[:4])
 
 
-def _loss_call(logits, value, pi, r, board, legal, scale, only_if_scaled, loss, d_logits, d_value):
+def _loss_call(logits, value, pi, r, board, legal, scale, only_if_scaled, total, parts, d_logits, d_value):
     n, actions = logits.shape
     work = torch.empty(_E.load_library().az_policy_loss_work(n, actions), dtype=torch.uint8, device=logits.device)
     _call("az_policy_loss", logits.device, *_row_args(logits, board, legal), value.data_ptr(),
-          int(value.dtype == torch.float32), pi.data_ptr(), r.data_ptr(), _ptr(scale), int(only_if_scaled), _ptr(loss),
-          _ptr(d_logits), _ptr(d_value), work.data_ptr())
+          int(value.dtype == torch.float32), pi.data_ptr(), r.data_ptr(), _ptr(scale), int(only_if_scaled), _ptr(total),
+          _ptr(parts), _ptr(d_logits), _ptr(d_value), work.data_ptr())
 
 
 class _LossFunction(torch.autograd.Function):
@@ -174,25 +180,27 @@ class _LossFunction(torch.autograd.Function):
                 for t, need in zip(inputs, ctx.needs_input_grad)]
 
     @staticmethod
-    def forward(ctx, logits, value, pi, r, board, legal):
-        loss = torch.empty(3, dtype=torch.float32, device=logits.device)
+    def forward(ctx, logits, value, pi, r, board, legal, want_parts):
+        total = torch.empty((), dtype=torch.float32, device=logits.device)
+        parts = torch.empty(2, dtype=torch.float32, device=logits.device) if want_parts else None
         d_logits, d_value = _LossFunction.buffers(ctx, logits, value)
-        _loss_call(logits, value, pi, r, board, legal, None, False, loss, d_logits, d_value)
+        _loss_call(logits, value, pi, r, board, legal, None, False, total, parts, d_logits, d_value)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, value, pi, r, board, legal)
         ctx.ready = (d_logits, d_value)
-        total, policy, val = loss.unbind()
-        ctx.mark_non_differentiable(policy, val)
-        return total, policy, val
+        if want_parts:
+            ctx.mark_non_differentiable(parts)
+        return total, parts
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g, _policy, _value):
+    def backward(ctx, g, _parts):
+        _once()
         logits, value, pi, r, board, legal = ctx.saved_tensors
         ready, ctx.ready = ctx.ready, None  # given away once: a second backward pass computes its own
         d_logits, d_value = ready or _LossFunction.buffers(ctx, logits, value)
-        _loss_call(logits, value, pi, r, board, legal, g.contiguous(), ready is not None, None, d_logits, d_value)
-        return d_logits, d_value, None, None, None, None
+        _loss_call(logits, value, pi, r, board, legal, g.contiguous(), ready is not None, None, None,
+                   d_logits, d_value)
+        return d_logits, d_value, None, None, None, None, None
 
 
 def loss(logits, value, pi, r, *, board=None, legal=None, parts=False):
@@ -220,5 +228,5 @@ def loss(logits, value, pi, r, *, board=None, legal=None, parts=False):
     if n == 0:
         zero = logits.sum(dtype=torch.float32) + value.sum(dtype=torch.float32)
         return (zero, zero.detach(), zero.detach()) if parts else zero
-    out = _LossFunction.apply(logits, value.contiguous(), pi.contiguous(), r.contiguous(), board, legal)
-    return out if parts else out[0]
+    total, two = _LossFunction.apply(logits, value.contiguous(), pi.contiguous(), r.contiguous(), board, legal, bool(parts))
+    return (total, two[0], two[1]) if parts else total

@@ -467,7 +467,7 @@ int az_policy_score_grad(int n, int actions, const void *d_logits, int dtype, lo
 /* The trainer's loss over n >= 1 records:  1/n sum_i sum_j pi_ij (log pi_ij - log p_ij) + 1/n sum_i (v_i - r_i)^2,
  * j over the legal cells (targets in masked cells are not looked at, 0 log 0 = 0, an empty row adds its value part only).
  *   d_value [n]: float32 (value_f32) or the logits' type; d_pi float32 [n][actions]; d_r float32 [n]
- *   d_loss [3] (may be NULL): total, policy part, value part
+ *   d_loss [1] (may be NULL): the total; d_parts [2] (may be NULL): policy part, value part
  *   d_dlogits [n][actions] (type of the logits), d_dvalue [n] (type of the values): gradients of the total times
  *   *d_scale (device float; NULL: 1); either may be NULL.  only_if_scaled: do nothing when *d_scale is 1 (the buffers
  *   hold the gradients of an earlier call with the same inputs and no scale).
@@ -475,8 +475,20 @@ int az_policy_score_grad(int n, int actions, const void *d_logits, int dtype, lo
 long long az_policy_loss_work(int n, int actions);
 int az_policy_loss(int n, int actions, const void *d_logits, int dtype, long long ld, const float *d_board,
                    const unsigned char *d_legal, long long ld_legal, const void *d_value, int value_f32, const float *d_pi,
-                   const float *d_r, const float *d_scale, int only_if_scaled, float *d_loss, void *d_dlogits,
+                   const float *d_r, const float *d_scale, int only_if_scaled, float *d_loss, float *d_parts, void *d_dlogits,
                    void *d_dvalue, void *d_work, void *stream);
+
+/* ---- orthogonalised weight updates (the trainer's side; the reference trains with Adam, src/train.py).
+ * Newton-Schulz steps on each of `count` matrices d_in[i] [rows][ld_in] (host array of device addresses, `dtype` AZ_F32 /
+ * AZ_BF16 / AZ_F16): X = G / |G|_F, then `steps` times X <- a X + (b A + c A^2) X with A = X X' (X' X for a matrix taller
+ * than wide) and (a, b, c) = (3.4445, -4.7750, 2.0315), to d_out[i] [rows][ld_out] in the same type (d_out[i] may be
+ * d_in[i]).  A matrix of zeros stays zero.  All of it in products of float32 precision whatever the type; the same
+ * inputs give the same bits.  d_work: az_muon_work(count, rows, cols) bytes, used by this call only; the device current
+ * at the call is the one of the pointers and of `stream`. */
+enum { AZ_MUON_MAX_DIM = 32768, AZ_MUON_MAX_CELLS = 1 << 28, AZ_MUON_MAX_STEPS = 20 };
+long long az_muon_work(int count, int rows, int cols);
+int az_muon_orthogonalise(int count, int rows, int cols, const void *const *d_in, long long ld_in, void *const *d_out,
+                          long long ld_out, int dtype, int steps, void *d_work, void *stream);
 
 #ifdef __cplusplus
 }

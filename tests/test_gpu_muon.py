@@ -1,0 +1,214 @@
+"""Orthogonalised updates (alphazero_amd.muon) against the definition in 64 bits.
+
+Tolerance: with u = 2^-24 a product of m x n matrices held in 22 bits (hi + lo, and the lo lo products left out) is off by
+at most about 8 u of its operands' sizes, entry errors of random sign; a step multiplies what an earlier one left by at
+most a = 3.4445, so the result's error is at most sum_{k < steps} a^k 8 u sqrt(terms that add up) of the input's
+size.  The input's size is |X_0|_F = 1 and errors of random sign spread over its m directions, so relative to the
+result's norm (about sqrt(rank)) the bound used is  a^(steps-1) * 1.41 * 32 u / sqrt(rank of the result)  plus 64 u for
+the later steps' own roundings; a result of 16 bits adds half a step of its type relative to its norm."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+ABC = (3.4445, -4.7750, 2.0315)
+
+
+def _exact(g, steps=5):
+    x = g.double()
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.transpose(-1, -2) if tall else x
+    norm = x.square().sum((-1, -2), keepdim=True).sqrt()
+    x = torch.where(norm > 0, x / norm, 0.0)
+    a, b, c = ABC
+    for _ in range(steps):
+        A = x @ x.transpose(-1, -2)
+        x = a * x + (b * A + c * (A @ A)) @ x
+    return x.transpose(-1, -2) if tall else x
+
+
+def _check(got, g, steps=5):
+    want = _exact(g.cpu(), steps)
+    assert got.shape == g.shape and got.dtype == g.dtype
+    off = (got.cpu().double() - want).flatten(-2).norm(dim=-1)
+    size = want.flatten(-2).norm(dim=-1)
+    tol = ABC[0] ** (steps - 1) * 1.41 * 32 * U + size * (64 * U + (torch.finfo(g.dtype).eps / 2 if g.dtype != torch.float32 else 0))
+    assert (off <= tol).all(), (off, tol, size)
+
+
+def _updates(shape, seed, scale=1e-3, rank=None):
+    gen = torch.Generator().manual_seed(seed)
+    rnd = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    m, n = shape[-2:]
+    if rank is None:
+        return rnd(*shape) * scale
+    return (rnd(*shape[:-1], rank) @ rnd(*shape[:-2], rank, n)) * scale
+
+
+SHAPES = [(1, 1), (1, 7), (7, 1), (2, 3), (16, 18), (16, 144), (144, 16), (31, 33), (32, 32), (33, 31), (63, 65), (64, 64), (64, 576),
+          (65, 63), (128, 100), (129, 127), (130, 1000), (200, 64), (256, 2304), (333, 1201), (512, 40), (640, 640), (17, 4100)]
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_against_the_definition(shape, dtype):
+    from alphazero_amd import muon
+
+    g = _updates(shape, 1, 1e-2).to(dtype).cuda()
+    _check(muon.orthogonalise(g), g)
+
+
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 6, 7, 10])
+@pytest.mark.parametrize("shape", [(16, 144), (100, 300), (300, 100)])
+def test_numbers_of_steps(steps, shape):
+    from alphazero_amd import muon
+
+    g = _updates(shape, steps).cuda()
+    _check(muon.orthogonalise(g, steps), g, min(steps, 7)) if steps <= 7 else None
+    if steps == 10:  # the singular values of a well conditioned update stay in the band that the polynomial maps to itself
+        s = torch.linalg.svdvals(muon.orthogonalise(g, 10).double().cpu())
+        assert 0.6 < s.min() and s.max() < 1.25
+
+
+@pytest.mark.parametrize("count", [1, 2, 7, 63, 64, 65, 130])
+def test_batches(count):
+    from alphazero_amd import muon
+
+    g = _updates((count, 16, 40), count).cuda()
+    got = muon.orthogonalise(g)
+    _check(got, g)
+    assert torch.equal(got[count // 2], muon.orthogonalise(g[count // 2]))  # a matrix's result is its own
+
+
+@pytest.mark.parametrize("shape", [(3, 130, 200), (2, 20, 50), (1, 700, 500)])
+def test_low_rank_sizes_and_zeros(shape):
+    from alphazero_amd import muon
+
+    for scale in (1e-30, 1e-3, 1e25):
+        g = _updates(shape, 3, 1.0, rank=4).cuda() * scale
+        _check(muon.orthogonalise(g), g)
+    g[0] = 0
+    got = muon.orthogonalise(g)
+    assert not got[0].any() and torch.isfinite(got).all()
+    if shape[0] > 1:
+        g[1, 3, 5] = math.nan
+        got = muon.orthogonalise(g)
+        assert got[1].isnan().all() and not got[0].any()
+        assert shape[0] < 3 or torch.isfinite(got[2]).all()
+
+
+def test_strides_lists_and_empty():
+    from alphazero_amd import muon
+
+    base = _updates((6, 50, 90), 5).cuda()
+    want = muon.orthogonalise(base[:, 3:43, 7:80].contiguous())
+    assert torch.equal(muon.orthogonalise(base[:, 3:43, 7:80]), want)
+    assert torch.equal(muon.orthogonalise(base[::2, 3:43, 7:80]), want[::2])
+    turned = base[:, 3:43, 7:80].transpose(1, 2).contiguous().transpose(1, 2)  # unit stride along the rows
+    assert torch.equal(muon.orthogonalise(turned), want)
+    assert torch.equal(muon.orthogonalise(base[:1, 3:43, 7:80].expand(4, 40, 73)), want[:1].expand(4, 40, 73))
+    conv = _updates((16, 16 * 9), 6).cuda().view(16, 16, 3, 3)
+    first = _updates((16, 2 * 9), 7).cuda().view(16, 2, 3, 3)
+    dense = _updates((30, 20), 8).cuda().bfloat16()
+    wide = base[0, :, :77]
+    got = muon.orthogonalise([conv, first, dense, conv * 2, wide, torch.empty(0, 4, device="cuda")])
+    assert [t.shape for t in got] == [conv.shape, first.shape, dense.shape, conv.shape, wide.shape, (0, 4)]
+    for g, t in ((conv, got[0]), (first, got[1]), (dense, got[2]), (wide, got[4])):
+        assert torch.equal(t.flatten(1), muon.orthogonalise(g.flatten(1)))
+        _check(t.flatten(1), g.flatten(1))
+    assert torch.equal(got[3], got[0])  # a factor of two does not change a single bit
+    assert muon.orthogonalise([]) == [] and muon.orthogonalise(base[:0]).shape == (0, 50, 90)
+    x = base[0].clone().requires_grad_()
+    assert not muon.orthogonalise(x).requires_grad
+
+
+def test_streams_and_graph_replay():
+    from alphazero_amd import muon
+
+    g = _updates((3, 100, 260), 9).cuda()
+    small = _updates((5, 16, 144), 10).cuda()
+    work = lambda: (muon.orthogonalise(g), muon.orthogonalise(small))  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        on_side = work()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(work(), on_side))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work()
+    for k in range(3):
+        g.add_(torch.randn_like(g) * 1e-3)
+        small.mul_(1.5).add_(1e-4)
+        want = [t.clone() for t in work()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+
+
+def test_optimiser_step_by_step():
+    from alphazero_amd import muon
+
+    torch.manual_seed(0)
+    w = [torch.nn.Parameter(torch.randn(16, 4, 3, 3, device="cuda")), torch.nn.Parameter(torch.randn(40, 10, device="cuda"))]
+    opt = muon.Muon(w, lr=0.1, momentum=0.9, weight_decay=0.01)
+    want = [p.detach().double().cpu() for p in w]
+    moments = [torch.zeros_like(p) for p in want]
+    for _ in range(3):
+        grads = [torch.randn_like(p) for p in w]
+        for p, g in zip(w, grads):
+            p.grad = g
+        opt.step()
+        for i, g in enumerate(grads):
+            g = g.double().cpu()
+            moments[i] = 0.9 * moments[i] + g
+            u = _exact((g + 0.9 * moments[i]).flatten(1)).view(g.shape)
+            want[i] = want[i] * (1 - 0.1 * 0.01) - 0.1 * max(1.0, g.shape[0] / g[0].numel()) ** 0.5 * u
+    for p, t in zip(w, want):
+        assert (p.detach().cpu().double() - t).norm() < 1e-5 * t.norm()
+    with pytest.raises(ValueError, match="two or more"):
+        muon.Muon([torch.nn.Parameter(torch.zeros(4))])
+
+
+def test_records_to_update_together():
+    # what a training program does: records -> symmetries and duplicates -> network -> loss -> gradients -> update
+    from alphazero_amd import augment, muon
+    from alphazero_amd.model import PolicyValueNet
+
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    n, S = 40, 7
+    board = torch.zeros(n, 2, S * S, device="cuda")
+    for i in range(n):
+        at = torch.randperm(S * S, generator=gen, device="cuda")[:2 * (i % 9)]
+        board[i, 0, at[::2]] = 1
+        board[i, 1, at[1::2]] = 1
+    board = board.view(n, 2, S, S)
+    pi = torch.rand(n, S * S, generator=gen, device="cuda") * (board.sum(1).flatten(1) == 0)
+    pi = pi / pi.sum(1, keepdim=True)
+    r = torch.where(torch.rand(n, generator=gen, device="cuda") < 0.5, 1.0, -1.0)
+    more = augment.rotations_device(board, pi, r)
+    board, pi, r = augment.unique_device(*[torch.cat(t) for t in zip((board, pi, r), more)])
+    torch.manual_seed(1)
+    net = PolicyValueNet(S).cuda()
+    weights, others = muon.Muon.weights_of(net)
+    assert len(weights) == 10 and all(p.dim() == 4 for p in weights)
+    opts = [muon.Muon(weights, lr=0.02), torch.optim.SGD(others, lr=0.02)]
+    before = [p.detach().clone() for p in weights]
+    net.loss(board, pi, r, mask_illegal=True).backward()
+    # the gradients of the masked loss, written with torch's own operators
+    grads = [p.grad.clone() for p in net.parameters()]
+    net.zero_grad()
+    value, logits = net.heads(board)
+    logp = torch.log_softmax(logits.masked_fill(board.sum(1).flatten(1) > 0, -1e30), 1)
+    (torch.nn.functional.kl_div(logp, pi, reduction="batchmean") + torch.nn.functional.mse_loss(value.view(-1), r)).backward()
+    for p, g in zip(net.parameters(), grads):
+        assert (p.grad - g).norm() <= 1e-3 * p.grad.norm() + 1e-6
+        p.grad = g
+    for opt in opts:
+        opt.step()
+    for p, b in zip(weights, before):
+        u = _exact((1.95 * p.grad).flatten(1).cpu()).view(p.shape)  # first step: m = g, u = g + 0.95 g
+        want = b.cpu().double() - 0.02 * max(1.0, p.shape[0] / p[0].numel()) ** 0.5 * u
+        assert (p.detach().cpu().double() - want).norm() < 1e-5 * want.norm()

@@ -1,0 +1,53 @@
+"""Refusals of the orthogonalised updates (alphazero_amd.muon and its C ABI), checked without a GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+from alphazero_amd import engine as E
+from alphazero_amd import muon
+
+G = torch.zeros(4, 9)
+
+
+@pytest.mark.parametrize("updates,steps,text", [
+    (G[0], 5, "a matrix, a batch"),
+    (G.view(1, 1, 4, 9), 5, "a matrix, a batch"),
+    (G.double(), 5, "float32, bfloat16 or float16"),
+    ([G, G.double()], 5, "float32, bfloat16 or float16"),
+    ([G, G[0]], 5, "two or more dimensions"),
+    ([G, 3], 5, "two or more dimensions"),
+    (G, 0, "steps must be"),
+    (G, 21, "steps must be"),
+    (G, 2.0, "steps must be"),
+    (torch.empty(1, 1).expand(32769, 1), 5, "at most 32768"),
+    (torch.empty(1, 1).expand(20000, 20000), 5, "cells"),
+    (G, 5, "no CPU path"),
+    ([G], 5, "no CPU path"),
+])
+def test_refuses(updates, steps, text):
+    with pytest.raises(ValueError, match=text):
+        muon.orthogonalise(updates, steps)
+
+
+def test_c_entry_refuses():
+    L = E.load_library()
+    one = (C.c_void_p * 1)(0x1000)  # never looked at: the sizes are refused first
+    none = (C.c_void_p * 1)(None)
+    call = lambda count=1, rows=4, cols=9, a=one, lda=9, b=one, ldb=9, dt=0, steps=5, work=0x1000: \
+        L.az_muon_orthogonalise(count, rows, cols, a, lda, b, ldb, dt, steps, work, None)  # noqa: E731
+    assert call(count=0) == 0
+    for bad in (dict(count=-1), dict(rows=0), dict(cols=0), dict(rows=32769), dict(rows=20000, cols=20000, lda=20000, ldb=20000),
+                dict(a=None), dict(b=None), dict(a=none), dict(b=none), dict(lda=8), dict(ldb=8), dict(dt=3), dict(steps=0),
+                dict(steps=21), dict(work=None)):
+        assert call(**bad) == E.ERR_ARG, bad
+    assert L.az_muon_work(1, 16, 144) > 0 and L.az_muon_work(0, 16, 144) == 0 and L.az_muon_work(1, 0, 5) == -1
+
+
+def test_optimiser_refuses():
+    p = torch.nn.Parameter(torch.zeros(3, 3))
+    for kw in (dict(lr=-1.0), dict(momentum=1.0), dict(weight_decay=-0.1), dict(steps=0)):
+        with pytest.raises(ValueError):
+            muon.Muon([p], **kw)
+    with pytest.raises(ValueError, match="two or more"):
+        muon.Muon([torch.nn.Parameter(torch.zeros(3))])

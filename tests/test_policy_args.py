@@ -63,7 +63,7 @@ def test_c_entries_refuse():
     assert L.az_policy_score_grad(1, 9, p, 0, 9, None, None, 0, None, p, 4, 1, p, p, None, p, p, None) == E.ERR_ARG
     assert L.az_policy_score_grad(1, 2000, p, 0, 2000, None, None, 0, p, p, 4, 1, p, None, None, p, p, None) == E.ERR_ARG
     loss = lambda n=1, scale=None, only=0, work=p: L.az_policy_loss(  # noqa: E731
-        n, 9, p, 0, 9, None, None, 0, p, 1, p, p, scale, only, p, p, p, work, None)
+        n, 9, p, 0, 9, None, None, 0, p, 1, p, p, scale, only, p, None, p, p, work, None)
     for bad in (dict(n=0), dict(only=1), dict(work=None)):
         assert loss(**bad) == E.ERR_ARG, bad
     assert L.az_policy_score_work(4, 400, 8) == 0 and L.az_policy_score_work(4, 4000, 8) > 0
