@@ -303,6 +303,254 @@ template <int BM, int BN, class T> __global__ __launch_bounds__(256, 2) void k_g
     }
 }
 
+// ---------------------------------------------------------------- small matrices: all steps in one launch
+//
+// A matrix of m <= 32 MT rows and n <= 256 NT columns belongs to one workgroup of 8 wavefronts and stays in registers:
+// a wavefront owns NT column tiles of 32 (lane l: column l mod 32; its registers: rows, in the order in which the matrix
+// instruction leaves a result).  In that order a tile is at once the operand of the next Q X: only Q's columns have to
+// be stored in the same order.  For the Gram matrix the tile is turned through LDS (rows to lanes), every wavefront adds
+// up its own columns and the eight partial sums meet in LDS in a fixed order.  Launches bound the general path here
+// (17 of them, 5 us each); this one is bound by the latency of 4 barriers a step and by one CU's matrix cores.
+constexpr int SMALL_WAVES = 8;
+
+// 16-byte piece of a row of M * 4 bytes: rows spread over the banks
+template <int M> __device__ __forceinline__ int bank(int r, int piece) { return M == 64 ? piece ^ (r & 15) : piece ^ ((r >> 1) & 7); }
+// first of the two pieces (hi, lo) of the 8 columns 16 c + 4 h + {0..3, 8..11} of a packed row
+__device__ __forceinline__ int slot(int c, int h) { return (c * 2 + h) * 2; }
+
+__device__ __forceinline__ void split8(const float *v, h8 &hi, h8 &lo)
+{
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        hi[i] = (_Float16)v[i];
+        lo[i] = (_Float16)(v[i] - (float)hi[i]);
+    }
+}
+
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+
+template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES, 2) void k_small(Ptrs p, Shape s, int steps)
+{
+    constexpr int M = 32 * MT, LD = M + 4, C = 2 * MT; // C: blocks of 16 rows
+    constexpr int AREA = M * M * 4 > 32 * LD * 4 ? M * M * 4 : 32 * LD * 4;
+    __shared__ __align__(16) char lds[SMALL_WAVES * AREA + M * M * 4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lr = lane & 31, half = lane >> 5;
+    char *area = lds + wave * AREA, *sA = lds, *sQ = lds + SMALL_WAVES * AREA;
+    const int tiles = (s.n + 31) / 32;
+
+    // X, and |X|
+    float x[NT][MT][16];
+    const T *g = (const T *)p.in[blockIdx.x];
+    double sum = 0.;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const int n = (t * SMALL_WAVES + wave) * 32 + lr;
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int m = i * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
+                const bool in = m < s.m && n < s.n;
+                const size_t at = s.tall ? (size_t)n * s.ld_in + m : (size_t)m * s.ld_in + n;
+                x[t][i][e] = in ? as_float(g[in ? at : 0]) : 0.f;
+            }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) sum = fma((double)x[t][i][e], (double)x[t][i][e], sum);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    if (lane == 0) ((double *)lds)[wave] = sum;
+    __syncthreads();
+    sum = 0.;
+#pragma unroll
+    for (int w = 0; w < SMALL_WAVES; w++) sum += ((double *)lds)[w];
+    __syncthreads();
+    const double scale = sum == 0. ? 0. : ldexp(1. / sqrt(sum), EXP_X);
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[t][i][e] = (float)((double)x[t][i][e] * scale);
+
+    for (int step = 0; step < steps; step++) {
+        // Gram matrix of this wavefront's columns, upper tiles
+        f16v gram[MT * (MT + 1) / 2];
+#pragma unroll
+        for (int q = 0; q < MT * (MT + 1) / 2; q++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) gram[q][e] = 0.f;
+        float *turn = (float *)area;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            if (t * SMALL_WAVES + wave >= tiles) continue;
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    *(float4 *)(turn + lr * LD + i * 32 + 2 * e + 4 * half) =
+                        make_float4(x[t][i][e], x[t][i][e + 1], x[t][i][e + 2], x[t][i][e + 3]);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            h8 hi[MT][2], lo[MT][2];
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+                float v[16];
+#pragma unroll
+                for (int q = 0; q < 16; q++) v[q] = turn[((q & 7) + 8 * half + 16 * (q >> 3)) * LD + i * 32 + lr];
+                split8(v, hi[i][0], lo[i][0]);
+                split8(v + 8, hi[i][1], lo[i][1]);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int i = 0, q = 0; i < MT; i++)
+#pragma unroll
+                for (int j = i; j < MT; j++, q++) {
+                    // the small products first, then the large ones on top, then one addition per 32 columns
+                    f16v acc;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) acc[e] = 0.f;
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo[i][c], hi[j][c], acc, 0, 0, 0);
+                        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi[i][c], lo[j][c], acc, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 2; c++) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi[i][c], hi[j][c], acc, 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 16; e++) gram[q][e] += acc[e];
+                }
+        }
+        // partial sums to the wavefront's own area, row c holding column c (the matrix is symmetric)
+#pragma unroll
+        for (int i = 0, q = 0; i < MT; i++)
+#pragma unroll
+            for (int j = i; j < MT; j++, q++) {
+                const int c = j * 32 + lr;
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const int r = i * 32 + 2 * e + 4 * half;
+                    *(float4 *)(area + c * M * 4 + bank<M>(c, r >> 2) * 16) = make_float4(gram[q][e], gram[q][e + 1], gram[q][e + 2], gram[q][e + 3]);
+                    if (i != j) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            *(float *)(area + (r + k) * M * 4 + bank<M>(r + k, c >> 2) * 16 + (c & 3) * 4) = gram[q][e + k];
+                    }
+                }
+            }
+        __syncthreads();
+        const int r = threadIdx.x / (M / 8), c16 = threadIdx.x % (M / 8) >> 1, h = threadIdx.x & 1;
+        const bool mine = threadIdx.x < M * M / 8;
+        float v[8];
+        if (mine) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = 0.f;
+#pragma unroll
+            for (int w = 0; w < SMALL_WAVES; w++) {
+                const char *row = lds + w * AREA + r * M * 4;
+                const float4 a = *(const float4 *)(row + bank<M>(r, c16 * 4 + h) * 16);
+                const float4 b = *(const float4 *)(row + bank<M>(r, c16 * 4 + h + 2) * 16);
+                v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+                v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = ldexpf(v[k], EXP_A - 2 * EXP_X);
+        }
+        __syncthreads();
+        if (mine) {
+            h8 hi, lo;
+            split8(v, hi, lo);
+            *(h8 *)(sA + r * M * 4 + bank<M>(r, slot(c16, h)) * 16) = hi;
+            *(h8 *)(sA + r * M * 4 + bank<M>(r, slot(c16, h) + 1) * 16) = lo;
+        }
+        __syncthreads();
+        // Q = a I + b A + c A^2, one 32 x 32 tile per wavefront
+        if (wave < MT * MT) {
+            const int i = wave / MT, j = wave % MT, ra = i * 32 + lr, rb = j * 32 + lr;
+            f16v acc;
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[e] = 0.f;
+            h8 ah[C], bh[C];
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                ah[c] = *(const h8 *)(sA + ra * M * 4 + bank<M>(ra, slot(c, half)) * 16);
+                bh[c] = *(const h8 *)(sA + rb * M * 4 + bank<M>(rb, slot(c, half)) * 16);
+                const h8 al = *(const h8 *)(sA + ra * M * 4 + bank<M>(ra, slot(c, half) + 1) * 16);
+                const h8 bl = *(const h8 *)(sA + rb * M * 4 + bank<M>(rb, slot(c, half) + 1) * 16);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh[c], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[c], bl, acc, 0, 0, 0);
+            }
+#pragma unroll
+            for (int c = 0; c < C; c++) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[c], bh[c], acc, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int row = i * 32 + 2 * e + 4 * half; // rows row..row+3 of column rb, stored as row rb
+                const int at = rb * M * 4 + (e >> 2 & 1) * 8, pc = slot(row >> 4, half);
+                const h4 hi = *(const h4 *)(sA + at + bank<M>(rb, pc) * 16), lo = *(const h4 *)(sA + at + bank<M>(rb, pc + 1) * 16);
+                h4 qh, ql;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    float f = acc[e + k] * (NS_C * 0x1p-18f); // 2^(EXP_Q - 2 EXP_A)
+                    f = fmaf((float)hi[k] + (float)lo[k], NS_B * 0x1p-4f, f);
+                    if (row + k == rb) f += NS_A * 0x1p10f;
+                    qh[k] = (_Float16)f;
+                    ql[k] = (_Float16)(f - (float)qh[k]);
+                }
+                *(h4 *)(sQ + at + bank<M>(rb, pc) * 16) = qh;
+                *(h4 *)(sQ + at + bank<M>(rb, pc + 1) * 16) = ql;
+            }
+        }
+        __syncthreads();
+        // X <- Q X
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            if (t * SMALL_WAVES + wave >= tiles) continue;
+            h8 xh[C], xl[C];
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+                split8(x[t][i], xh[2 * i], xl[2 * i]);
+                split8(x[t][i] + 8, xh[2 * i + 1], xl[2 * i + 1]);
+            }
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+                const int rq = i * 32 + lr;
+                f16v acc;
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[e] = 0.f;
+                h8 qh[C];
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    qh[c] = *(const h8 *)(sQ + rq * M * 4 + bank<M>(rq, slot(c, half)) * 16);
+                    const h8 ql = *(const h8 *)(sQ + rq * M * 4 + bank<M>(rq, slot(c, half) + 1) * 16);
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql, xh[c], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[c], xl[c], acc, 0, 0, 0);
+                }
+#pragma unroll
+                for (int c = 0; c < C; c++) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[c], xh[c], acc, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 16; e++) x[t][i][e] = acc[e] * 0x1p-10f; // 2^-EXP_Q
+            }
+        }
+    }
+    T *out = (T *)p.out[blockIdx.x];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const int n = (t * SMALL_WAVES + wave) * 32 + lr;
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int m = i * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
+                if (m < s.m && n < s.n) put(out + (s.tall ? (size_t)n * s.ld_out + m : (size_t)m * s.ld_out + n), x[t][i][e] * 0x1p-15f);
+            }
+    }
+}
+static_assert(EXP_X == 15 && EXP_A == 14 && EXP_Q == 10, "the powers of two written out in k_small");
+
 // ---------------------------------------------------------------- host side
 
 int launch_ok() { return hipGetLastError() == hipSuccess ? AZ_OK : AZ_ERR_HIP; }
@@ -369,6 +617,29 @@ bool shape_ok(int count, int rows, int cols, int dtype, int steps)
 {
     return count >= 0 && rows >= 1 && cols >= 1 && rows <= AZ_MUON_MAX_DIM && cols <= AZ_MUON_MAX_DIM &&
            (long long)rows * cols <= AZ_MUON_MAX_CELLS && dtype >= AZ_F32 && dtype <= AZ_F16 && steps >= 1 && steps <= AZ_MUON_MAX_STEPS;
+}
+
+// Matrices that one workgroup holds in registers (128 of them per lane at most)
+bool is_small(const Shape &s) { return (s.m <= 32 && s.n <= 2048) || (s.m <= 64 && s.n <= 768); }
+
+int run_small(int batch, const Shape &s, int dtype, int steps, const Ptrs &p, hipStream_t st)
+{
+    const int nt = (s.n + 255) / 256;
+    by_type(dtype, [&](auto *d) {
+        using T = std::remove_pointer_t<decltype(d)>;
+        const auto go = [&](auto *kernel) { hipLaunchKernelGGL(kernel, dim3(batch), dim3(64 * SMALL_WAVES), 0, st, p, s, steps); };
+        if (s.m <= 32) {
+            if (nt <= 1) go(k_small<1, 1, T>);
+            else if (nt <= 2) go(k_small<1, 2, T>);
+            else if (nt <= 4) go(k_small<1, 4, T>);
+            else go(k_small<1, 8, T>);
+        } else {
+            if (nt <= 1) go(k_small<2, 1, T>);
+            else if (nt <= 2) go(k_small<2, 2, T>);
+            else go(k_small<2, 3, T>);
+        }
+    });
+    return launch_ok();
 }
 
 int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *work, hipStream_t st)
@@ -468,6 +739,7 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
 // large fill the chip one by one).
 int batch_of(const Shape &s, int count)
 {
+    if (is_small(s)) return count < MAX_BATCH ? count : MAX_BATCH;
     const size_t one = plan_of(s, 1).total;
     long long most = (long long)(((size_t)1 << 30) / one);
     if (most < 1) most = 1;
@@ -484,7 +756,7 @@ long long az_muon_work(int count, int rows, int cols)
     if (!shape_ok(count, rows, cols, AZ_F32, 1)) return -1;
     if (count == 0) return 0;
     const Shape s = shape_of(rows, cols);
-    return (long long)plan_of(s, batch_of(s, count)).total;
+    return is_small(s) ? 0 : (long long)plan_of(s, batch_of(s, count)).total;
 }
 
 int az_muon_orthogonalise(int count, int rows, int cols, const void *const *d_in, long long ld_in, void *const *d_out,
@@ -492,12 +764,14 @@ int az_muon_orthogonalise(int count, int rows, int cols, const void *const *d_in
 {
     if (!shape_ok(count, rows, cols, dtype, steps) || ld_in < cols || ld_out < cols) return AZ_ERR_ARG;
     if (count == 0) return AZ_OK;
-    if (!d_in || !d_out || !d_work) return AZ_ERR_ARG;
+    if (!d_in || !d_out) return AZ_ERR_ARG;
     for (int i = 0; i < count; i++)
         if (!d_in[i] || !d_out[i]) return AZ_ERR_ARG;
     Shape s = shape_of(rows, cols);
     s.ld_in = ld_in;
     s.ld_out = ld_out;
+    const bool small = is_small(s);
+    if (!small && !d_work) return AZ_ERR_ARG;
     const int batch = batch_of(s, count);
     for (int at = 0; at < count; at += batch) {
         const int n = count - at < batch ? count - at : batch;
@@ -506,7 +780,7 @@ int az_muon_orthogonalise(int count, int rows, int cols, const void *const *d_in
             p.in[i] = d_in[at + i];
             p.out[i] = d_out[at + i];
         }
-        const int rc = run_batch(n, s, dtype, steps, p, (char *)d_work, (hipStream_t)stream);
+        const int rc = small ? run_small(n, s, dtype, steps, p, (hipStream_t)stream) : run_batch(n, s, dtype, steps, p, (char *)d_work, (hipStream_t)stream);
         if (rc != AZ_OK) return rc;
     }
     return AZ_OK;

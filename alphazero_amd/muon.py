@@ -8,7 +8,7 @@ import ctypes as C
 import torch
 
 from . import engine as _E
-from .policy import TYPES, _call, _refuse
+from .policy import TYPES, _call, _ptr, _refuse
 
 MAX_DIM, MAX_CELLS, MAX_STEPS = 32768, 1 << 28, 20  # AZ_MUON_MAX_*
 
@@ -31,9 +31,10 @@ def _run(inputs, outputs, rows, cols, ld, dtype, device, steps):
     """inputs, outputs: device addresses of matrices of one shape, rows `ld` (outputs: cols) elements apart."""
     count = len(inputs)
     addresses = C.c_void_p * count
-    work = torch.empty(_E.load_library().az_muon_work(count, rows, cols), dtype=torch.uint8, device=device)
+    size = _E.load_library().az_muon_work(count, rows, cols)
+    work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     _call("az_muon_orthogonalise", device, count, rows, cols, addresses(*inputs), ld, addresses(*outputs), cols,
-          TYPES[dtype], steps, work.data_ptr())
+          TYPES[dtype], steps, _ptr(work))
 
 
 def _rows_apart(x):

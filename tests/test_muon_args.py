@@ -39,9 +39,9 @@ def test_c_entry_refuses():
     assert call(count=0) == 0
     for bad in (dict(count=-1), dict(rows=0), dict(cols=0), dict(rows=32769), dict(rows=20000, cols=20000, lda=20000, ldb=20000),
                 dict(a=None), dict(b=None), dict(a=none), dict(b=none), dict(lda=8), dict(ldb=8), dict(dt=3), dict(steps=0),
-                dict(steps=21), dict(work=None)):
+                dict(steps=21), dict(rows=100, cols=100, lda=100, ldb=100, work=None)):
         assert call(**bad) == E.ERR_ARG, bad
-    assert L.az_muon_work(1, 16, 144) > 0 and L.az_muon_work(0, 16, 144) == 0 and L.az_muon_work(1, 0, 5) == -1
+    assert L.az_muon_work(1, 100, 144) > 0 and L.az_muon_work(1, 16, 144) == 0 and L.az_muon_work(0, 16, 144) == 0 and L.az_muon_work(1, 0, 5) == -1
 
 
 def test_optimiser_refuses():
