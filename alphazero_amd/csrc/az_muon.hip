@@ -82,7 +82,7 @@ __device__ __forceinline__ void pack8(char *p, const float (&v)[8])
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         hi[i] = (_Float16)v[i];
-        lo[i] = (_Float16)(v[i] - (float)hi[i]);
+        lo[i] = (_Float16)fmaf(-1.f, (float)hi[i], v[i]);
     }
     *(h8 *)p = hi;
     *(h8 *)(p + 16) = lo;
@@ -307,9 +307,9 @@ template <int BM, int BN, class T> __global__ __launch_bounds__(256, 2) void k_g
 //
 // A matrix of m <= 32 MT rows and n <= 256 NT columns belongs to one workgroup of 8 wavefronts and stays in registers:
 // a wavefront owns NT column tiles of 32 (lane l: column l mod 32; its registers: rows, in the order in which the matrix
-// instruction leaves a result).  In that order a tile is at once the operand of the next Q X: only Q's columns have to
-// be stored in the same order.  For the Gram matrix the tile is turned through LDS (rows to lanes), every wavefront adds
-// up its own columns and the eight partial sums meet in LDS in a fixed order.  Launches bound the general path here
+// instruction leaves a result), as hi and lo halves.  In that order a tile is at once the operand of the next Q X: only
+// Q's columns have to be stored in the same order.  For the Gram matrix the tile is turned through LDS (rows to lanes)
+// by transposing reads, every wavefront adds up its own columns and the eight partial sums meet in LDS in a fixed order.  Launches bound the general path here
 // (17 of them, 5 us each); this one is bound by the latency of 4 barriers a step and by one CU's matrix cores.
 constexpr int SMALL_WAVES = 8;
 
@@ -323,60 +323,78 @@ __device__ __forceinline__ void split8(const float *v, h8 &hi, h8 &lo)
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         hi[i] = (_Float16)v[i];
-        lo[i] = (_Float16)(v[i] - (float)hi[i]);
+        lo[i] = (_Float16)fmaf(-1.f, (float)hi[i], v[i]); // exact (one instruction: an operand may be float16)
     }
 }
 
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 
+// 8 columns of a row from two transposing LDS reads of 4
+typedef short s4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ h8 turned(const char *a, const char *b)
+{
+    union { struct { s4 a, b; } s; h8 h; } u;
+    u.s.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)a);
+    u.s.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)b);
+    return u.h;
+}
+__device__ __forceinline__ int row_of(int r) { return (r & ~12) | (r & 4) << 1 | (r & 8) >> 1; }
+
 template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES, 2) void k_small(Ptrs p, Shape s, int steps)
 {
-    constexpr int M = 32 * MT, LD = M + 4, C = 2 * MT; // C: blocks of 16 rows
-    constexpr int AREA = M * M * 4 > 32 * LD * 4 ? M * M * 4 : 32 * LD * 4;
+    constexpr int M = 32 * MT, LD = M + 8, C = 2 * MT; // C: blocks of 16 rows
+    constexpr int TURN = 32 * LD * 2;                  // one half (hi or lo) of a tile, [column][row], rows 16 bytes apart
+    constexpr int AREA = M * M * 4 > 2 * TURN ? M * M * 4 : 2 * TURN;
     __shared__ __align__(16) char lds[SMALL_WAVES * AREA + M * M * 4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lr = lane & 31, half = lane >> 5;
     char *area = lds + wave * AREA, *sA = lds, *sQ = lds + SMALL_WAVES * AREA;
     const int tiles = (s.n + 31) / 32;
 
-    // X, and |X|
-    float x[NT][MT][16];
-    const T *g = (const T *)p.in[blockIdx.x];
-    double sum = 0.;
+    // X and |X|.  A lane's registers hold, of each block of 16 rows, rows 4 half + {0..3, 8..11}: hi and lo, 8 each
+    h8 xh[NT][C], xl[NT][C];
+    {
+        float x[NT][C][8];
+        const T *g = (const T *)p.in[blockIdx.x];
+        const long long pm = s.tall ? 1 : s.ld_in, pn = s.tall ? s.ld_in : 1;
+        double sum = 0.;
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
-        const int n = (t * SMALL_WAVES + wave) * 32 + lr;
+        for (int t = 0; t < NT; t++) {
+            const int n = (t * SMALL_WAVES + wave) * 32 + lr;
+            const T *col = g + min(n, s.n - 1) * pn;
 #pragma unroll
-        for (int i = 0; i < MT; i++)
+            for (int c = 0; c < C; c++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int m = i * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
-                const bool in = m < s.m && n < s.n;
-                const size_t at = s.tall ? (size_t)n * s.ld_in + m : (size_t)m * s.ld_in + n;
-                x[t][i][e] = in ? as_float(g[in ? at : 0]) : 0.f;
+                for (int e = 0; e < 8; e++) {
+                    const int m = c * 16 + 8 * (e >> 2) + 4 * half + (e & 3);
+                    const float v = as_float(col[min(m, s.m - 1) * pm]); // (no branch: all loads are in flight together)
+                    x[t][c][e] = m < s.m && n < s.n ? v : 0.f;
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) sum = fma((double)x[t][c][e], (double)x[t][c][e], sum);
+#pragma unroll
+        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+        if (lane == 0) ((double *)lds)[wave] = sum;
+        __syncthreads();
+        sum = 0.;
+#pragma unroll
+        for (int w = 0; w < SMALL_WAVES; w++) sum += ((double *)lds)[w];
+        __syncthreads();
+        const double scale = sum == 0. ? 0. : ldexp(1. / sqrt(sum), EXP_X);
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[t][c][e] = (float)((double)x[t][c][e] * scale);
+                split8(x[t][c], xh[t][c], xl[t][c]);
             }
     }
-#pragma unroll
-    for (int t = 0; t < NT; t++)
-#pragma unroll
-        for (int i = 0; i < MT; i++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) sum = fma((double)x[t][i][e], (double)x[t][i][e], sum);
-#pragma unroll
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-    if (lane == 0) ((double *)lds)[wave] = sum;
-    __syncthreads();
-    sum = 0.;
-#pragma unroll
-    for (int w = 0; w < SMALL_WAVES; w++) sum += ((double *)lds)[w];
-    __syncthreads();
-    const double scale = sum == 0. ? 0. : ldexp(1. / sqrt(sum), EXP_X);
-#pragma unroll
-    for (int t = 0; t < NT; t++)
-#pragma unroll
-        for (int i = 0; i < MT; i++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) x[t][i][e] = (float)((double)x[t][i][e] * scale);
 
     for (int step = 0; step < steps; step++) {
         // Gram matrix of this wavefront's columns, upper tiles
@@ -385,26 +403,26 @@ template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES
         for (int q = 0; q < MT * (MT + 1) / 2; q++)
 #pragma unroll
             for (int e = 0; e < 16; e++) gram[q][e] = 0.f;
-        float *turn = (float *)area;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             if (t * SMALL_WAVES + wave >= tiles) continue;
+            // turned through LDS: a transposing read hands lane l of 16 the 4 columns of place l of a block of 16 rows, so
+            // the operand's rows come with bits 2 and 3 of their number exchanged (row_of)
 #pragma unroll
-            for (int i = 0; i < MT; i++)
-#pragma unroll
-                for (int e = 0; e < 16; e += 4)
-                    *(float4 *)(turn + lr * LD + i * 32 + 2 * e + 4 * half) =
-                        make_float4(x[t][i][e], x[t][i][e + 1], x[t][i][e + 2], x[t][i][e + 3]);
+            for (int c = 0; c < C; c++) {
+                *(h8 *)(area + (lr * LD + c * 16 + half * 8) * 2) = xh[t][c];
+                *(h8 *)(area + TURN + (lr * LD + c * 16 + half * 8) * 2) = xl[t][c];
+            }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             h8 hi[MT][2], lo[MT][2];
 #pragma unroll
-            for (int i = 0; i < MT; i++) {
-                float v[16];
+            for (int i = 0; i < MT; i++)
 #pragma unroll
-                for (int q = 0; q < 16; q++) v[q] = turn[((q & 7) + 8 * half + 16 * (q >> 3)) * LD + i * 32 + lr];
-                split8(v, hi[i][0], lo[i][0]);
-                split8(v + 8, hi[i][1], lo[i][1]);
-            }
+                for (int c = 0; c < 2; c++) {
+                    const int n = c * 16 + half * 8 + (lr >> 2 & 3), at = (n * LD + i * 32 + (lr >> 4) * 16 + (lr & 3) * 4) * 2;
+                    hi[i][c] = turned(area + at, area + at + 4 * LD * 2);
+                    lo[i][c] = turned(area + TURN + at, area + TURN + at + 4 * LD * 2);
+                }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
             for (int i = 0, q = 0; i < MT; i++)
@@ -430,10 +448,10 @@ template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES
         for (int i = 0, q = 0; i < MT; i++)
 #pragma unroll
             for (int j = i; j < MT; j++, q++) {
-                const int c = j * 32 + lr;
+                const int c = row_of(j * 32 + lr);
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) {
-                    const int r = i * 32 + 2 * e + 4 * half;
+                    const int r = row_of(i * 32 + 2 * e + 4 * half);
                     *(float4 *)(area + c * M * 4 + bank<M>(c, r >> 2) * 16) = make_float4(gram[q][e], gram[q][e + 1], gram[q][e + 2], gram[q][e + 3]);
                     if (i != j) {
 #pragma unroll
@@ -509,12 +527,7 @@ template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             if (t * SMALL_WAVES + wave >= tiles) continue;
-            h8 xh[C], xl[C];
-#pragma unroll
-            for (int i = 0; i < MT; i++) {
-                split8(x[t][i], xh[2 * i], xl[2 * i]);
-                split8(x[t][i] + 8, xh[2 * i + 1], xl[2 * i + 1]);
-            }
+            float x[C][8];
 #pragma unroll
             for (int i = 0; i < MT; i++) {
                 const int rq = i * 32 + lr;
@@ -526,26 +539,30 @@ template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES
                 for (int c = 0; c < C; c++) {
                     qh[c] = *(const h8 *)(sQ + rq * M * 4 + bank<M>(rq, slot(c, half)) * 16);
                     const h8 ql = *(const h8 *)(sQ + rq * M * 4 + bank<M>(rq, slot(c, half) + 1) * 16);
-                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql, xh[c], acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[c], xl[c], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql, xh[t][c], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[c], xl[t][c], acc, 0, 0, 0);
                 }
 #pragma unroll
-                for (int c = 0; c < C; c++) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[c], xh[c], acc, 0, 0, 0);
+                for (int c = 0; c < C; c++) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[c], xh[t][c], acc, 0, 0, 0);
 #pragma unroll
-                for (int e = 0; e < 16; e++) x[t][i][e] = acc[e] * 0x1p-10f; // 2^-EXP_Q
+                for (int e = 0; e < 16; e++) x[2 * i + (e >> 3)][e & 7] = acc[e] * 0x1p-10f; // 2^-EXP_Q
             }
+#pragma unroll
+            for (int c = 0; c < C; c++) split8(x[c], xh[t][c], xl[t][c]);
         }
     }
     T *out = (T *)p.out[blockIdx.x];
+    const long long pm = s.tall ? 1 : s.ld_out, pn = s.tall ? s.ld_out : 1;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
         const int n = (t * SMALL_WAVES + wave) * 32 + lr;
 #pragma unroll
-        for (int i = 0; i < MT; i++)
+        for (int c = 0; c < C; c++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int m = i * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
-                if (m < s.m && n < s.n) put(out + (s.tall ? (size_t)n * s.ld_out + m : (size_t)m * s.ld_out + n), x[t][i][e] * 0x1p-15f);
+            for (int e = 0; e < 8; e++) {
+                const int m = c * 16 + 8 * (e >> 2) + 4 * half + (e & 3);
+                const float v = ((float)xh[t][c][e] + (float)xl[t][c][e]) * 0x1p-15f; // 2^-EXP_X
+                if (m < s.m && n < s.n) put(out + n * pn + m * pm, v);
             }
     }
 }
