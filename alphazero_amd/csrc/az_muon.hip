@@ -29,7 +29,7 @@ namespace {
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr int EXP_X = 15, EXP_A = 14, EXP_Q = 10; // stored number = value * 2^EXP
 constexpr int MAX_BATCH = 64;                     // matrices per launch (their addresses travel as kernel arguments)
-constexpr int NORM_PARTS = 64;                    // partial sums of squares per matrix, at most
+constexpr int NORM_PARTS = 256;                   // partial sums of squares per matrix, at most
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f16v __attribute__((ext_vector_type(16)));
@@ -59,18 +59,23 @@ struct Shape {
 template <class T> __global__ __launch_bounds__(256) void k_norm(Ptrs p, Shape s, int parts, double *sums)
 {
     const T *g = (const T *)p.in[blockIdx.y];
-    double acc = 0.;
-    for (int i = blockIdx.x * 4 + (threadIdx.x >> 6); i < s.rows; i += parts * 4) {
+    double acc[4] = {0., 0., 0., 0.};
+    // a wavefront takes pieces of 256 cells of a row
+    const int pieces = (s.cols + 255) / 256;
+    for (long long u = blockIdx.x * 4 + (threadIdx.x >> 6); u < (long long)s.rows * pieces; u += parts * 4) {
+        const int i = (int)(u / pieces), j = (int)(u - (long long)i * pieces) * 256 + (threadIdx.x & 63);
         const T *row = g + (size_t)i * s.ld_in;
-        for (int j = threadIdx.x & 63; j < s.cols; j += 64) {
-            const double v = (double)as_float(row[j]);
-            acc = fma(v, v, acc);
-        }
-    }
+        float v[4];
 #pragma unroll
-    for (int o = 32; o; o >>= 1) acc += __shfl_xor(acc, o);
+        for (int k = 0; k < 4; k++) v[k] = as_float(row[min(j + 64 * k, s.cols - 1)]);
+#pragma unroll
+        for (int k = 0; k < 4; k++) acc[k] = j + 64 * k < s.cols ? fma((double)v[k], (double)v[k], acc[k]) : acc[k];
+    }
+    double sum = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
     __shared__ double s_w[4];
-    if ((threadIdx.x & 63) == 0) s_w[threadIdx.x >> 6] = acc;
+    if ((threadIdx.x & 63) == 0) s_w[threadIdx.x >> 6] = sum;
     __syncthreads();
     if (threadIdx.x == 0) sums[(size_t)blockIdx.y * NORM_PARTS + blockIdx.x] = (s_w[0] + s_w[1]) + (s_w[2] + s_w[3]);
 }
@@ -94,41 +99,45 @@ __device__ __forceinline__ void unpack8(const char *p, float (&v)[8])
     for (int i = 0; i < 8; i++) v[i] = (float)hi[i] + (float)lo[i];
 }
 
-// G / |G| packed as X [mp][np] and as its transpose [np][mp]; one 64 x 64 tile of G per workgroup
-template <class T> __global__ __launch_bounds__(256) void k_split(Ptrs p, Shape s, int parts, const double *sums, char *X, char *XT)
+// X' = the packed transpose of G / |G| (G itself, row by row, when it is tall), [np][mp]; one 64 x 64 tile of G per workgroup
+template <class T> __global__ __launch_bounds__(256) void k_split(Ptrs p, Shape s, int parts, const double *sums, char *XT)
 {
     __shared__ float t[64][65];
     __shared__ double s_scale;
     const int b = blockIdx.z;
     const T *g = (const T *)p.in[b];
+    const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+    float v[16]; // all loads are in flight while the sum is taken
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+        const int r = r0 + (threadIdx.x >> 6) + 4 * k, c = c0 + (threadIdx.x & 63);
+        v[k] = as_float(g[(size_t)min(r, s.rows - 1) * s.ld_in + min(c, s.cols - 1)]);
+        v[k] = r < s.rows && c < s.cols ? v[k] : 0.f;
+    }
     if (threadIdx.x < 64) {
-        double sum = (int)threadIdx.x < parts ? sums[(size_t)b * NORM_PARTS + threadIdx.x] : 0.;
+        double sum = 0.;
+#pragma unroll
+        for (int i = 0; i < NORM_PARTS; i += 64) sum += i + (int)threadIdx.x < parts ? sums[(size_t)b * NORM_PARTS + i + threadIdx.x] : 0.;
 #pragma unroll
         for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
         if (threadIdx.x == 0) s_scale = sum == 0. ? 0. : ldexp(1. / sqrt(sum), EXP_X);
     }
     __syncthreads();
     const double scale = s_scale;
-    const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
-    for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-        const int r = e >> 6, c = e & 63;
-        const bool in = r0 + r < s.rows && c0 + c < s.cols;
-        t[r][c] = in ? (float)((double)as_float(g[(size_t)(r0 + r) * s.ld_in + c0 + c]) * scale) : 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+        const int r = (threadIdx.x >> 6) + 4 * k, c = threadIdx.x & 63;
+        t[s.tall ? r : c][s.tall ? c : r] = (float)((double)v[k] * scale);
     }
     __syncthreads();
-    // G row-major is X when wide and X' when tall
-    char *same = s.tall ? XT : X, *turned = s.tall ? X : XT;
-    const int rp = s.tall ? s.np : s.mp, cp = s.tall ? s.mp : s.np; // padded rows and columns of G
-    const size_t size = (size_t)s.mp * s.np * 4;
+    const int n0 = s.tall ? r0 : c0, m0 = s.tall ? c0 : r0;
+    char *out = XT + b * ((size_t)s.mp * s.np * 4);
     for (int e = threadIdx.x; e < 64 * 8; e += 256) {
-        const int r = e >> 3, c = (e & 7) * 8;
-        float v[8];
+        const int n = e >> 3, m = (e & 7) * 8;
+        float w[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = t[r][c + i];
-        if (r0 + r < rp && c0 + c < cp) pack8(same + b * size + ((size_t)(r0 + r) * cp + c0 + c) * 4, v);
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = t[c + i][r];
-        if (c0 + r < cp && r0 + c < rp) pack8(turned + b * size + ((size_t)(c0 + r) * rp + r0 + c) * 4, v);
+        for (int i = 0; i < 8; i++) w[i] = t[n][m + i];
+        if (n0 + n < s.np && m0 + m < s.mp) pack8(out + ((size_t)(n0 + n) * s.mp + m0 + m) * 4, w);
     }
 }
 
@@ -138,14 +147,13 @@ struct Gemm {
     size_t sA, sB;      // bytes from one matrix of the batch to the next
     int pitchA, pitchB; // bytes per row
     int K;
-    int tiles_m, tiles_n, symmetric; // symmetric: upper tiles only, each written to both of its places
+    int tiles, tiles_m, tiles_n; // tiles per matrix
+    int symmetric;      // upper tiles only, each written to both of its places
     float alpha, beta, gamma;
     const char *E;      // packed, same shape as D; or NULL
-    size_t sE;
-    char *D, *DT;       // packed result [M][N] and / or its transpose [N][M]; or NULL
-    size_t sD;
-    int pitchD, pitchDT;
-    int user;           // write p.out[] (rows of D are rows of G, or columns when s.tall)
+    size_t sE, sD;
+    char *D;            // packed result [M][N]; NULL: to p.out[], as G (D is its transpose, or itself when it is tall)
+    int pitchD;
 };
 
 // 16 bytes per lane straight into LDS; the wavefront's 64 lanes fill 1 KB from `lds` on in lane order
@@ -155,49 +163,115 @@ __device__ __forceinline__ void load_lds(const char *g, char *lds)
                                      (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
 }
 
+// 8 numbers of K for one row of an operand, from two transposing LDS reads of 4: of 16 lanes, lane 4 j + q hands over 4
+// neighbouring columns (place q) of row j, and lane l receives column l of the four rows
+typedef short s4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ h8 turned(const char *a, const char *b)
+{
+    union { struct { s4 a, b; } s; h8 h; } u;
+    u.s.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)a);
+    u.s.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)b);
+    return u.h;
+}
+
 constexpr int BK = 32;              // K per stage: 128 bytes of a packed row
 // place of 16-byte piece c of row r within the row's 128 bytes: 16 lanes that read the same piece of 16 rows touch
 // all 64 banks
 __device__ __forceinline__ int place(int r, int c) { return c ^ ((r >> 1) & 7); }
+// the same for rows of K: the four rows of a transposing read, 64 bytes of each, touch all 64 banks
+__device__ __forceinline__ int place_k(int k, int c) { return c ^ ((k & 1) | (k & 2) << 2); }
 
-// BM x BN results per workgroup of 4 wavefronts (2 x 2); per stage and wavefront (BM/64) (BN/64) 2 x 3 matrix
+constexpr int BAND = 8; // tiles are taken in bands of 8 rows, column by column: 64 neighbours share 8 + 8 panels
+__device__ __forceinline__ void tile_at(int i, const Gemm &a, int &ti, int &tj)
+{
+    for (int first = 0;; first += BAND) {
+        const int rows = min(BAND, a.tiles_m - first);
+        if (!a.symmetric) {
+            const int n = rows * a.tiles_n;
+            if (i < n) {
+                ti = first + i % rows;
+                tj = i / rows;
+                return;
+            }
+            i -= n;
+            continue;
+        }
+        const int corner = rows * (rows + 1) / 2, n = corner + rows * (a.tiles_n - first - rows);
+        if (i >= n) {
+            i -= n;
+            continue;
+        }
+        if (i < corner) {
+            int j = 0;
+            while (i > j) i -= ++j;
+            ti = first + i;
+            tj = first + j;
+        } else {
+            i -= corner;
+            ti = first + i % rows;
+            tj = first + rows + i / rows;
+        }
+        return;
+    }
+}
+
+// BM x BN results per workgroup of KS groups of 4 wavefronts (2 x 2); per stage and wavefront (BM/64) (BN/64) 2 x 3 matrix
 // instructions 32x32x16 on (BM/64 + BN/64) 4 LDS reads.  Two stages in LDS: the next one loads while this one is used.
-template <int BM, int BN, class T> __global__ __launch_bounds__(256, 2) void k_gemm(Gemm a, Ptrs p, Shape s)
+// The groups take every KS-th stage of K and add up at the end: more wavefronts per CU where tiles are few.
+// TURN: A and B are given as [K][M] and [K][N] (the Gram matrix from X'), and the LDS reads transpose.
+template <int BM, int BN, int KS, bool TURN, class T>
+__global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs p, Shape s)
 {
     constexpr int FM = BM / 64, FN = BN / 64; // 32 x 32 blocks of a wavefront
     constexpr int STAGE = (BM + BN) * 128;
-    constexpr int TILE = BM * (BN + 4) * 4;
-    __shared__ __align__(16) char lds[2 * STAGE > TILE ? 2 * STAGE : TILE];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int b = blockIdx.y;
-    // neighbouring tiles share operands: give each of the 8 XCDs (workgroups go round them) a run of tiles
-    int tile;
+    constexpr int LT = BN + 1;
+    constexpr int TILE = BM * LT * 4;
+    constexpr int THREADS = 256 * KS;
+    __shared__ __align__(16) char lds_all[2 * KS * STAGE > TILE ? 2 * KS * STAGE : TILE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+    const int group = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    char *lds = lds_all + group * 2 * STAGE;
+    // workgroups go round the 8 XCDs: each XCD gets a run of neighbouring tiles, which share operands in its L2
+    int b, ti, tj;
     {
         const int n = gridDim.x, x = blockIdx.x & 7, i = blockIdx.x >> 3, per = n >> 3, rest = n & 7;
-        tile = x * per + min(x, rest) + i;
+        const int item = x * per + min(x, rest) + i;
+        b = item / a.tiles;
+        tile_at(item - b * a.tiles, a, ti, tj);
     }
-    int ti, tj;
-    if (a.symmetric) {
-        ti = 0;
-        while (tile >= a.tiles_n - ti) tile -= a.tiles_n - ti++;
-        tj = ti + tile;
-    } else {
-        ti = tile / a.tiles_n;
-        tj = tile - ti * a.tiles_n;
-    }
-    const char *A = a.A + b * a.sA + (size_t)ti * BM * a.pitchA;
-    const char *B = a.B + b * a.sB + (size_t)tj * BN * a.pitchB;
+    const char *A = a.A + b * a.sA + (TURN ? (size_t)ti * BM * 4 : (size_t)ti * BM * a.pitchA);
+    const char *B = a.B + b * a.sB + (TURN ? (size_t)tj * BN * 4 : (size_t)tj * BN * a.pitchB);
 
-    constexpr int LOADS = (BM + BN) / 8 / 4; // 8-row loads per wavefront and stage
+    constexpr int LOADS = (BM + BN) / 8 / 4; // 1 KB loads per wavefront and stage
     const char *src[LOADS];
     int dst[LOADS];
+    size_t next_a = 128, next_b = 128; // from stage to stage
+    if (TURN) {
+        next_a = (size_t)BK * a.pitchA;
+        next_b = (size_t)BK * a.pitchB;
+    }
 #pragma unroll
     for (int l = 0; l < LOADS; l++) {
-        const int r8 = (l * 4 + wave) * 8, r = r8 + (lane >> 3);
-        const int c = place(r, lane & 7);
-        src[l] = r8 < BM ? A + (size_t)r * a.pitchA + c * 16 : B + (size_t)(r - BM) * a.pitchB + c * 16;
-        dst[l] = r8 * 128;
+        const int kb = l * 4 + wave; // KB of the stage
+        dst[l] = kb * 1024;
+        if (TURN) {
+            constexpr int PA = BM / 4, PB = BN / 4; // 16-byte pieces per row of K
+            if (kb < BM / 8) {
+                const int k = kb * 64 / PA + lane / PA;
+                src[l] = A + (size_t)k * a.pitchA + place_k(k, lane % PA) * 16;
+            } else {
+                const int k = (kb - BM / 8) * 64 / PB + lane / PB;
+                src[l] = B + (size_t)k * a.pitchB + place_k(k, lane % PB) * 16;
+            }
+        } else {
+            const int r = kb * 8 + (lane >> 3), c = place(r, lane & 7);
+            src[l] = kb * 8 < BM ? A + (size_t)r * a.pitchA + c * 16 : B + (size_t)(r - BM) * a.pitchB + c * 16;
+        }
     }
+    const auto load_stage = [&](int k, char *to) {
+#pragma unroll
+        for (int l = 0; l < LOADS; l++) load_lds(src[l] + (size_t)k * (l * 4 < BM / 8 ? next_a : next_b), to + dst[l]);
+    };
     // the small products have accumulators of their own: added to the large ones they would cost a rounding each
     // (three times the error of one step)
     f16v acc[FM][FN], low[FM][FN];
@@ -210,32 +284,48 @@ template <int BM, int BN, class T> __global__ __launch_bounds__(256, 2) void k_g
     const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
     const int lr = lane & 31, half = lane >> 5;
     const int stages = a.K / BK;
-#pragma unroll
-    for (int l = 0; l < LOADS; l++) load_lds(src[l], lds + dst[l]);
-    for (int k = 0; k < stages; k++) {
+    if (group < stages) load_stage(group, lds);
+    const int rounds = (stages + KS - 1) / KS;
+    for (int k = 0; k < rounds; k++) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // this wavefront's part of stage k has arrived
         __syncthreads();                                 // all of it has; nobody reads the other buffer any more
         const char *cur = lds + (k & 1) * STAGE;
-        if (k + 1 < stages) {
-            char *next = lds + ((k + 1) & 1) * STAGE;
-#pragma unroll
-            for (int l = 0; l < LOADS; l++) load_lds(src[l] + (size_t)(k + 1) * 128, next + dst[l]);
-        }
+        const int after = (k + 1) * KS + group;
+        if (after < stages) load_stage(after, lds + ((k + 1) & 1) * STAGE);
+        if (KS > 1 && k * KS + group >= stages) break; // (the last round; this group's share is done)
 #pragma unroll
         for (int ks = 0; ks < 2; ks++) {
             h8 ah[FM], al[FM], bh[FN], bl[FN];
-            const int c = (ks * 2 + half) * 2;
+            if (TURN) {
+                const int q = lane & 3, kk = ks * 16 + half * 8 + (lane >> 2 & 3), f = place_k(kk, 0), up = (lane >> 4 & 1) * 4 + (q & 2);
 #pragma unroll
-            for (int i = 0; i < FM; i++) {
-                const int r = wm + i * 32 + lr;
-                ah[i] = *(const h8 *)(cur + r * 128 + place(r, c) * 16);
-                al[i] = *(const h8 *)(cur + r * 128 + place(r, c + 1) * 16);
-            }
+                for (int i = 0; i < FM; i++) {
+                    const char *at = cur + kk * BM * 4 + (q & 1) * 8;
+                    const int c = (wm + i * 32) / 4 + up;
+                    ah[i] = turned(at + (c ^ f) * 16, at + 4 * BM * 4 + (c ^ f) * 16);
+                    al[i] = turned(at + ((c + 1) ^ f) * 16, at + 4 * BM * 4 + ((c + 1) ^ f) * 16);
+                }
 #pragma unroll
-            for (int j = 0; j < FN; j++) {
-                const int r = BM + wn + j * 32 + lr;
-                bh[j] = *(const h8 *)(cur + r * 128 + place(r, c) * 16);
-                bl[j] = *(const h8 *)(cur + r * 128 + place(r, c + 1) * 16);
+                for (int j = 0; j < FN; j++) {
+                    const char *at = cur + BM * 128 + kk * BN * 4 + (q & 1) * 8;
+                    const int c = (wn + j * 32) / 4 + up;
+                    bh[j] = turned(at + (c ^ f) * 16, at + 4 * BN * 4 + (c ^ f) * 16);
+                    bl[j] = turned(at + ((c + 1) ^ f) * 16, at + 4 * BN * 4 + ((c + 1) ^ f) * 16);
+                }
+            } else {
+                const int c = (ks * 2 + half) * 2;
+#pragma unroll
+                for (int i = 0; i < FM; i++) {
+                    const int r = wm + i * 32 + lr;
+                    ah[i] = *(const h8 *)(cur + r * 128 + place(r, c) * 16);
+                    al[i] = *(const h8 *)(cur + r * 128 + place(r, c + 1) * 16);
+                }
+#pragma unroll
+                for (int j = 0; j < FN; j++) {
+                    const int r = BM + wn + j * 32 + lr;
+                    bh[j] = *(const h8 *)(cur + r * 128 + place(r, c) * 16);
+                    bl[j] = *(const h8 *)(cur + r * 128 + place(r, c + 1) * 16);
+                }
             }
 #pragma unroll
             for (int i = 0; i < FM; i++)
@@ -249,33 +339,39 @@ template <int BM, int BN, class T> __global__ __launch_bounds__(256, 2) void k_g
     }
     // the tile through LDS, so that every write is a whole group of 8 whichever way the result is stored
     __syncthreads();
-    float *t = (float *)lds;
-    constexpr int LT = BN + 4;
+    float *t = (float *)lds_all;
 #pragma unroll
-    for (int i = 0; i < FM; i++)
+    for (int g = KS - 1; g >= 0; g--) { // the groups one after the other: a fixed order
+        if (group == g) {
 #pragma unroll
-        for (int j = 0; j < FN; j++)
+            for (int i = 0; i < FM; i++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int r = wm + i * 32 + (e >> 2) * 8 + half * 4 + (e & 3), c = wn + j * 32 + lr;
-                t[r * LT + c] = (acc[i][j][e] + low[i][j][e]) * a.alpha;
-            }
-    __syncthreads();
+                for (int j = 0; j < FN; j++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const int r = wm + i * 32 + (e >> 2) * 8 + half * 4 + (e & 3), c = wn + j * 32 + lr;
+                        const float v = (acc[i][j][e] + low[i][j][e]) * a.alpha;
+                        t[r * LT + c] = g == KS - 1 ? v : v + t[r * LT + c];
+                    }
+        }
+        __syncthreads();
+    }
     const int row0 = ti * BM, col0 = tj * BN;
-    if (a.user) {
+    if (!a.D) { // rows of the result: n, columns: m
         T *out = (T *)p.out[b];
-        for (int e = threadIdx.x; e < BM * BN; e += 256) {
-            if (!s.tall) {
+        for (int e = threadIdx.x; e < BM * BN; e += THREADS) {
+            if (s.tall) {
                 const int r = e / BN, c = e % BN;
-                if (row0 + r < s.m && col0 + c < s.n) put(out + (size_t)(row0 + r) * s.ld_out + col0 + c, t[r * LT + c]);
+                if (row0 + r < s.n && col0 + c < s.m) put(out + (size_t)(row0 + r) * s.ld_out + col0 + c, t[r * LT + c]);
             } else {
                 const int c = e / BM, r = e % BM;
-                if (row0 + r < s.m && col0 + c < s.n) put(out + (size_t)(col0 + c) * s.ld_out + row0 + r, t[r * LT + c]);
+                if (row0 + r < s.n && col0 + c < s.m) put(out + (size_t)(col0 + c) * s.ld_out + row0 + r, t[r * LT + c]);
             }
         }
         return;
     }
-    for (int e = threadIdx.x; e < BM * BN / 8; e += 256) {
+    char *D = a.D + b * a.sD;
+    for (int e = threadIdx.x; e < BM * BN / 8; e += THREADS) {
         const int r = e / (BN / 8), c = e % (BN / 8) * 8;
         float v[8];
 #pragma unroll
@@ -290,16 +386,16 @@ template <int BM, int BN, class T> __global__ __launch_bounds__(256, 2) void k_g
                 t[r * LT + c + i] = v[i];
             }
         }
-        if (a.D) pack8(a.D + b * a.sD + at, v);
+        pack8(D + at, v);
     }
-    if (!a.DT || (a.symmetric && ti == tj)) return;
+    if (!a.symmetric || ti == tj) return;
     __syncthreads();
-    for (int e = threadIdx.x; e < BM * BN / 8; e += 256) {
+    for (int e = threadIdx.x; e < BM * BN / 8; e += THREADS) {
         const int c = e / (BM / 8), r = e % (BM / 8) * 8;
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = t[(r + i) * LT + c];
-        pack8(a.DT + b * a.sD + (size_t)(col0 + c) * a.pitchDT + (size_t)(row0 + r) * 4, v);
+        pack8(D + (size_t)(col0 + c) * a.pitchD + (size_t)(row0 + r) * 4, v);
     }
 }
 
@@ -329,15 +425,6 @@ __device__ __forceinline__ void split8(const float *v, h8 &hi, h8 &lo)
 
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 
-// 8 columns of a row from two transposing LDS reads of 4
-typedef short s4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ h8 turned(const char *a, const char *b)
-{
-    union { struct { s4 a, b; } s; h8 h; } u;
-    u.s.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)a);
-    u.s.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)b);
-    return u.h;
-}
 __device__ __forceinline__ int row_of(int r) { return (r & ~12) | (r & 4) << 1 | (r & 8) >> 1; }
 
 template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES, 2) void k_small(Ptrs p, Shape s, int steps)
@@ -604,30 +691,36 @@ Plan plan_of(const Shape &s, int batch)
     p.x = (size_t)s.mp * s.np * 4;
     p.mm = (size_t)s.mp * s.mp * 4;
     p.sums = (size_t)batch * NORM_PARTS * sizeof(double);
-    p.total = p.sums + batch * (3 * p.x + 5 * p.mm);
+    p.total = p.sums + batch * (2 * p.x + 5 * p.mm);
     return p;
 }
 
 // launches D = alpha A B' + ... over `batch` matrices
-void gemm(Gemm a, int M, int N, int batch, int dtype, const Ptrs &p, const Shape &s, hipStream_t st)
+void gemm(Gemm a, int M, int N, bool turn, int batch, int dtype, const Ptrs &p, const Shape &s, hipStream_t st)
 {
     // 128 x 128 tiles halve the operand traffic of 64 x 64 ones, but a launch should have a workgroup for every CU
     const auto tiles = [&](int t) { return a.symmetric ? (long long)(M / t) * (M / t + 1) / 2 : (long long)(M / t) * (N / t); };
     const bool big = M % 128 == 0 && N % 128 == 0 && tiles(128) * batch >= 256;
     const int t = big ? 128 : 64;
+    const long long groups = tiles(t) * batch;
+    a.tiles = (int)tiles(t);
     a.tiles_m = M / t;
     a.tiles_n = N / t;
-    const dim3 grid((unsigned)tiles(t), batch), block(256);
-    if (!a.user) {
-        if (big) hipLaunchKernelGGL((k_gemm<128, 128, float>), grid, block, 0, st, a, p, s);
-        else hipLaunchKernelGGL((k_gemm<64, 64, float>), grid, block, 0, st, a, p, s);
-        return;
-    }
-    by_type(dtype, [&](auto *d) {
+    // workgroups that leave CUs with one or two of them get more wavefronts each
+    const int ks = big ? 1 : groups <= 256 ? 4 : groups <= 512 ? 2 : 1;
+    const dim3 grid((unsigned)groups), block(256 * ks);
+    const auto go = [&](auto *kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, a, p, s); };
+    const auto run = [&](auto turn, auto *d) {
         using T = std::remove_pointer_t<decltype(d)>;
-        if (big) hipLaunchKernelGGL((k_gemm<128, 128, T>), grid, block, 0, st, a, p, s);
-        else hipLaunchKernelGGL((k_gemm<64, 64, T>), grid, block, 0, st, a, p, s);
-    });
+        constexpr bool TURN = decltype(turn)::value;
+        if (big) go(k_gemm<128, 128, 1, TURN, T>);
+        else if (ks == 4) go(k_gemm<64, 64, 4, TURN, T>);
+        else if (ks == 2) go(k_gemm<64, 64, 2, TURN, T>);
+        else go(k_gemm<64, 64, 1, TURN, T>);
+    };
+    if (turn) run(std::true_type(), (float *)nullptr);
+    else if (a.D) run(std::false_type(), (float *)nullptr);
+    else by_type(dtype, [&](auto *d) { run(std::false_type(), d); });
 }
 
 bool shape_ok(int count, int rows, int cols, int dtype, int steps)
@@ -663,32 +756,33 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
 {
     const Plan pl = plan_of(s, batch);
     double *sums = (double *)work;
-    char *X = work + pl.sums, *XT = X + batch * pl.x, *YT = XT + batch * pl.x;
+    char *XT = work + pl.sums, *YT = XT + batch * pl.x;
     char *mm[5];
     for (int i = 0; i < 5; i++) mm[i] = YT + batch * pl.x + i * batch * pl.mm;
-    int parts = (s.rows + 15) / 16;
-    if (parts > NORM_PARTS) parts = NORM_PARTS;
-    const int rp = s.tall ? s.np : s.mp, cp = s.tall ? s.mp : s.np;
+    // workgroups per matrix: eight pieces for each wavefront, or what fills the chip
+    long long parts_l = ((long long)s.rows * ((s.cols + 255) / 256) + 31) / 32;
+    const int parts = (int)(parts_l > NORM_PARTS ? NORM_PARTS : parts_l);
+    const int rp = s.tall ? s.np : s.mp, cp = s.tall ? s.mp : s.np; // padded rows and columns of G
     by_type(dtype, [&](auto *d) {
         using T = std::remove_pointer_t<decltype(d)>;
         hipLaunchKernelGGL((k_norm<T>), dim3(parts, batch), dim3(256), 0, st, p, s, parts, sums);
-        hipLaunchKernelGGL((k_split<T>), dim3((cp + 63) / 64, (rp + 63) / 64, batch), dim3(256), 0, st, p, s, parts, (const double *)sums, X, XT);
+        hipLaunchKernelGGL((k_split<T>), dim3((cp + 63) / 64, (rp + 63) / 64, batch), dim3(256), 0, st, p, s, parts, (const double *)sums, XT);
     });
     const auto two = [](int e) { return ldexpf(1.f, e); };
-    const int px = s.np * 4, pm = s.mp * 4;
+    const int pm = s.mp * 4;
     // a symmetric m x m product of two packed ones, 2^ex * 2^ey in the accumulator, stored with 2^eo
     const auto square = [&](const char *x, int ex, const char *y, int ey, char *out, int eo, float f = 1.f, const char *E = nullptr,
                             float beta = 0.f, float gamma = 0.f) {
         Gemm g = {};
         g.A = x; g.B = y;
         g.sA = g.sB = g.sE = g.sD = pl.mm;
-        g.pitchA = g.pitchB = g.pitchD = g.pitchDT = pm;
+        g.pitchA = g.pitchB = g.pitchD = pm;
         g.K = s.mp;
         g.symmetric = 1;
         g.alpha = f * two(eo - ex - ey);
         g.E = E; g.beta = beta; g.gamma = gamma;
-        g.D = g.DT = out;
-        gemm(g, s.mp, s.mp, batch, dtype, p, s, st);
+        g.D = out;
+        gemm(g, s.mp, s.mp, false, batch, dtype, p, s, st);
     };
     // Steps per group.  Results of 16 bits (half a step: 2^-9, 2^-12) have room for three.  For float32 groups of two
     // keep the error where single steps have it and pay where X is much wider than high: at n = 4 m they leave 47
@@ -700,16 +794,16 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
         char *A = mm[0], *T = mm[1], *Q = mm[2], *W = mm[3], *V = mm[4];
         {
             Gemm g = {};
-            g.A = g.B = X;
+            g.A = g.B = XT;
             g.sA = g.sB = pl.x;
-            g.pitchA = g.pitchB = px;
+            g.pitchA = g.pitchB = pm;
             g.K = s.np;
             g.symmetric = 1;
             g.alpha = two(EXP_A - 2 * EXP_X);
             g.sD = pl.mm;
-            g.pitchD = g.pitchDT = pm;
-            g.D = g.DT = A;
-            gemm(g, s.mp, s.mp, batch, dtype, p, s, st);
+            g.pitchD = pm;
+            g.D = A;
+            gemm(g, s.mp, s.mp, true, batch, dtype, p, s, st);
         }
         const auto poly = [&](char *out) { // a I + b A + c A^2
             square(A, EXP_A, A, EXP_A, out, EXP_Q, NS_C, A, NS_B * two(EXP_Q - EXP_A), NS_A * two(EXP_Q));
@@ -730,21 +824,18 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
         }
         const char *total = k == 1 ? W : Q;
         left -= k;
-        Gemm g = {};
-        g.A = total; g.B = XT;
-        g.sA = pl.mm; g.sB = pl.x;
+        Gemm g = {}; // X' <- X' Q
+        g.A = XT; g.B = total;
+        g.sA = pl.x; g.sB = pl.mm;
         g.pitchA = g.pitchB = pm;
         g.K = s.mp;
-        g.user = left == 0;
         g.alpha = two((left ? EXP_X : 0) - EXP_Q - EXP_X);
-        if (left) { // X is not read here, its transpose is
+        if (left) {
             g.sD = pl.x;
-            g.D = X;
-            g.pitchD = px;
-            g.DT = YT;
-            g.pitchDT = pm;
+            g.D = YT;
+            g.pitchD = pm;
         }
-        gemm(g, s.mp, s.np, batch, dtype, p, s, st);
+        gemm(g, s.np, s.mp, false, batch, dtype, p, s, st);
         char *t = XT;
         XT = YT;
         YT = t;
