@@ -22,8 +22,9 @@ namespace {
 constexpr int WAVES = 4;                 // wavefronts per workgroup
 constexpr int SHORT_MAX = 1024;          // longest row held in registers (16 cells per lane)
 constexpr int MAX_ACTIONS = 1 << 24;
-constexpr int LONG_R = 8;                // cells per lane and step of a long row
+constexpr int LONG_R = 16;               // cells per lane and step of a long row
 constexpr int LONG_STEP = 64 * LONG_R;
+constexpr int MAX_CHUNKS = 256;          // chunks per row
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float NINF = -INFINITY;
 
@@ -173,17 +174,36 @@ __device__ __forceinline__ void best_insert(Best &b, float v, int i, int lane) /
     b.i = lane < pos ? b.i : lane == pos ? i : ui;
 }
 
-// cells of one register, whose indices all come after those already listed
-__device__ __forceinline__ void best_offer(Best &b, float x, int index, int k, int lane)
+// The cells of a step, whose indices (first + 64 r + lane) all come after those already listed.  Of many candidates only
+// those not below the k-th largest of the 64 lane maxima can be among the k best, few more than k as a rule; those are
+// put into the list one by one, in the order of their indices.
+template <int R> __device__ __forceinline__ void best_offer(Best &b, const float (&x)[R], int first, int k, int lane)
 {
     float limit = lane_of(b.v, k - 1);
-    unsigned long long todo = __ballot(x > limit);
-    while (todo) {
-        const int l = __ffsll((unsigned long long)todo) - 1;
-        best_insert(b, lane_of(x, l), __builtin_amdgcn_readlane(index, l), lane);
-        limit = lane_of(b.v, k - 1);
-        todo &= todo - 1;
-        todo &= __ballot(x > limit);
+    float top = x[0]; // (NaN is ignored by fmaxf, and never above the limit)
+#pragma unroll
+    for (int r = 1; r < R; r++) top = fmaxf(top, x[r]);
+    const unsigned long long some = __ballot(top > limit);
+    if (!some) return;
+    float least = NINF;
+    if (__popcll(some) > k) {
+        float v = top > limit ? top : NINF;
+        for (int i = 1; i < k; i++) {
+            const unsigned long long at = __ballot(v == wave_max(v));
+            if (lane == __ffsll(at) - 1) v = NINF;
+        }
+        least = wave_max(v);
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        unsigned long long todo = __ballot(x[r] > limit && x[r] >= least);
+        while (todo) {
+            const int l = __ffsll(todo) - 1;
+            best_insert(b, lane_of(x[r], l), first + r * 64 + l, lane);
+            limit = lane_of(b.v, k - 1);
+            todo &= todo - 1;
+            todo &= __ballot(x[r] > limit);
+        }
     }
 }
 
@@ -548,10 +568,7 @@ template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_parts(Ro
                 X += w == 0.f ? 0.f : w * d;
             }
         }
-        if (o.top) {
-#pragma unroll
-            for (int r = 0; r < LONG_R; r++) best_offer(best, x[r], j0 + r * 64 + lane, o.top, lane);
-        }
+        if (o.top) best_offer<LONG_R>(best, x, j0, o.top, lane);
     }
     Part out = {M, wave_sum(S), wave_sum(U), wave_sum(W), wave_sum(E), wave_sum(X)};
     if (lane == 0) o.part[unit] = out;
@@ -588,12 +605,19 @@ __device__ __forceinline__ Part join_parts(const Part *part, int count, int lane
     return Part{M, wave_sum(S), wave_sum(U), wave_sum(W), wave_sum(E), wave_sum(X)};
 }
 
-// one wavefront per row: outputs of az_policy_score from the chunks' numbers and lists
-template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_score(Rows a, Chunks c, LongOut w, ScoreOut o)
+// one wavefront per row: outputs of az_policy_score from the chunks' numbers and lists.  The lists are merged in LDS: a
+// lane holds the heads of every 64th list, each round takes the largest head (of equal ones the lowest index)
+template <class T> __global__ __launch_bounds__(64) void k_long_score(Rows a, Chunks c, LongOut w, ScoreOut o)
 {
-    const int lane = threadIdx.x & 63;
-    const long long row = (long long)blockIdx.x * WAVES + (threadIdx.x >> 6);
-    if (row >= a.n) return;
+    extern __shared__ float s_list[]; // [chunks][top] values, then indices
+    const int lane = threadIdx.x;
+    const long long row = blockIdx.x;
+    const int cells = c.count * o.top;
+    int *s_index = (int *)(s_list + cells);
+    for (int i = lane; i < cells; i += 64) {
+        s_list[i] = w.list_v[(size_t)row * cells + i];
+        s_index[i] = w.list_i[(size_t)row * cells + i];
+    }
     const Part t = join_parts(w.part + (size_t)row * c.count, c.count, lane);
     const bool live = t.S != 0.f;
     const float logS = live ? logf(t.S) : 0.f;
@@ -615,18 +639,56 @@ template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_score(Ro
         }
         o.logp[(size_t)row * o.m + lane] = r;
     }
-    if (o.top) {
-        Best best = {NINF, -1};
-        for (int i = 0; i < c.count; i++) { // chunks in order: of equal values the lowest index stays in front
-            const size_t at = ((size_t)row * c.count + i) * o.top;
-            const float v = lane < o.top ? w.list_v[at + lane] : NINF;
-            const int idx = lane < o.top ? w.list_i[at + lane] : -1;
-            best_offer(best, v, idx, o.top, lane);
+    if (!o.top) return;
+    __syncthreads();
+    constexpr int HEADS = MAX_CHUNKS / 64;
+    float head[HEADS];
+    int next[HEADS]; // where the head's successor stands
+#pragma unroll
+    for (int h = 0; h < HEADS; h++) {
+        const int list = h * 64 + lane;
+        head[h] = list < c.count ? s_list[list * o.top] : NINF;
+        next[h] = list * o.top + 1;
+    }
+    float mine_v = NINF;
+    int mine_i = -1;
+    for (int k = 0; k < o.top; k++) {
+        float v = head[0];
+        int from = 0;
+#pragma unroll
+        for (int h = 1; h < HEADS; h++) {
+            from = head[h] > v ? h : from; // (lists in the order of their indices: of equal heads the first)
+            v = head[h] > v ? head[h] : v;
         }
-        if (lane < o.top) {
-            o.top_logp[(size_t)row * o.top + lane] = best.i < 0 ? NINF : best.v - t.M - logS;
-            o.top_moves[(size_t)row * o.top + lane] = best.i;
+        const float best = wave_max(v);
+        if (best == NINF) break;
+        // of the lanes with this value the one whose list comes first holds the lowest index
+        int list = v == best ? from * 64 + lane : 0x7fffffff;
+        unsigned long long who = __ballot(v == best);
+        if (who & (who - 1)) {
+#pragma unroll
+            for (int s = 32; s; s >>= 1) list = min(list, __shfl_xor(list, s));
+        } else {
+            list = __builtin_amdgcn_readlane(list, __ffsll(who) - 1);
         }
+        int at = 0;
+#pragma unroll
+        for (int h = 0; h < HEADS; h++) {
+            if (list == h * 64 + lane) {
+                at = next[h] - 1;
+                head[h] = next[h] < (list + 1) * o.top ? s_list[next[h]] : NINF;
+                next[h]++;
+            }
+        }
+        at = __builtin_amdgcn_readlane(at, list & 63);
+        if (lane == k) {
+            mine_v = best;
+            mine_i = s_index[at];
+        }
+    }
+    if (lane < o.top) {
+        o.top_logp[(size_t)row * o.top + lane] = mine_i < 0 ? NINF : mine_v - t.M - logS;
+        o.top_moves[(size_t)row * o.top + lane] = mine_i;
     }
 }
 
@@ -740,14 +802,15 @@ int grid_of(long long units)
     return (int)(b < GRID_MAX ? b : GRID_MAX);
 }
 
-// Chunks of a long row: about 4096 wavefronts over all rows (16 per CU) when the rows alone are fewer, chunks of at least
-// two steps, at most 256 chunks (what one wavefront joins in four turns).
-Chunks chunks_of(int n, int A)
+// Chunks of a long row: about 8192 wavefronts over all rows (32 per CU) when the rows alone are fewer, chunks of at least
+// one step, at most as many as one wavefront can merge (their lists in 32 KB of LDS).
+Chunks chunks_of(int n, int A, int top)
 {
-    long long want = n > 0 ? (4096 + n - 1) / n : 1;
-    const long long most = (A + 2 * LONG_STEP - 1) / (2 * LONG_STEP);
+    long long want = n > 0 ? (8192 + n - 1) / n : 1;
+    const long long most = (A + LONG_STEP - 1) / LONG_STEP;
+    const long long fit = top > 16 ? MAX_CHUNKS / 2 : MAX_CHUNKS;
     if (want > most) want = most;
-    if (want > 256) want = 256;
+    if (want > fit) want = fit;
     if (want < 1) want = 1;
     const long long len = ((A + want - 1) / want + LONG_STEP - 1) / LONG_STEP * LONG_STEP;
     return Chunks{(int)len, (int)((A + len - 1) / len)};
@@ -761,7 +824,7 @@ bool rows_ok(const Rows &a, int dtype)
 
 size_t long_work(int n, int A, int top)
 {
-    const Chunks c = chunks_of(n, A);
+    const Chunks c = chunks_of(n, A, top);
     return (size_t)n * c.count * (sizeof(Part) + 8 * (size_t)top);
 }
 
@@ -823,7 +886,7 @@ int az_policy_score(int n, int actions, const void *d_logits, int dtype, long lo
         return launch_ok();
     }
     if (!d_work) return AZ_ERR_ARG;
-    const Chunks c = chunks_of(n, actions);
+    const Chunks c = chunks_of(n, actions, top);
     LongOut w = {};
     w.part = (Part *)d_work;
     w.list_v = (float *)(w.part + (size_t)n * c.count);
@@ -834,7 +897,7 @@ int az_policy_score(int n, int actions, const void *d_logits, int dtype, long lo
     by_type(dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
         hipLaunchKernelGGL((k_long_parts<T>), dim3((unsigned)((units + WAVES - 1) / WAVES)), block, 0, st, a, c, w);
-        hipLaunchKernelGGL((k_long_score<T>), dim3((n + WAVES - 1) / WAVES), block, 0, st, a, c, w, o);
+        hipLaunchKernelGGL((k_long_score<T>), dim3(n), dim3(64), (size_t)c.count * top * 8, st, a, c, w, o);
     });
     return launch_ok();
 }
@@ -853,7 +916,7 @@ int az_policy_score_grad(int n, int actions, const void *d_logits, int dtype, lo
     const ScoreGrad o = {d_moves, move_bytes, m, d_g_logp, d_g_entropy, d_entropy, d_stats, d_mask, d_dlogits};
     const dim3 block(64 * WAVES);
     const hipStream_t st = (hipStream_t)stream;
-    const Chunks c = chunks_of(n, actions);
+    const Chunks c = chunks_of(n, actions, 0);
     const long long units = (long long)n * c.count;
     if (actions > SHORT_MAX && (units + WAVES - 1) / WAVES > 0x7fffffffll) return AZ_ERR_ARG;
     by_type(dtype, [&](auto *t) {
@@ -896,7 +959,7 @@ int az_policy_loss(int n, int actions, const void *d_logits, int dtype, long lon
             });
         });
     } else {
-        const Chunks c = chunks_of(n, actions);
+        const Chunks c = chunks_of(n, actions, 0);
         const long long units = (long long)n * c.count;
         if ((units + WAVES - 1) / WAVES > 0x7fffffffll) return AZ_ERR_ARG;
         LongOut w = {};

@@ -4,6 +4,7 @@ optimiser that applies them to a network's weight matrices.
 The HIP kernels (csrc/az_muon.hip, reached through the C ABI) run on torch's current stream of the tensors' device; they
 allocate through torch, wait for nothing and can be captured into a graph."""
 import ctypes as C
+import functools
 
 import torch
 
@@ -11,6 +12,11 @@ from . import engine as _E
 from .policy import TYPES, _call, _ptr, _refuse
 
 MAX_DIM, MAX_CELLS, MAX_STEPS = 32768, 1 << 28, 20  # AZ_MUON_MAX_*
+
+
+@functools.lru_cache(1024)
+def _work(count, rows, cols):
+    return _E.load_library().az_muon_work(count, rows, cols)
 
 
 def _check(rows, cols, dtype, steps):
@@ -31,9 +37,9 @@ def _run(inputs, outputs, rows, cols, ld, dtype, device, steps):
     """inputs, outputs: device addresses of matrices of one shape, rows `ld` (outputs: cols) elements apart."""
     count = len(inputs)
     addresses = C.c_void_p * count
-    size = _E.load_library().az_muon_work(count, rows, cols)
+    size = _work(count, rows, cols)
     work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    _call("az_muon_orthogonalise", device, count, rows, cols, addresses(*inputs), ld, addresses(*outputs), cols,
+    _call("az_muon_orthogonalise", device.index, count, rows, cols, addresses(*inputs), ld, addresses(*outputs), cols,
           TYPES[dtype], steps, _ptr(work))
 
 
@@ -60,7 +66,7 @@ def orthogonalise(updates, steps=5):
         rows, cols = updates.shape[-2:]
         _check(rows, cols, updates.dtype, steps)
         _on_gpu([updates])
-        out = torch.empty(updates.shape, dtype=updates.dtype, device=updates.device)
+        out = updates.new_empty(updates.shape)
         if out.numel():
             x, ld = _rows_apart(updates)
             size = x.element_size()
