@@ -92,13 +92,6 @@ __device__ __forceinline__ void pack8(char *p, const float (&v)[8])
     *(h8 *)p = hi;
     *(h8 *)(p + 16) = lo;
 }
-__device__ __forceinline__ void unpack8(const char *p, float (&v)[8])
-{
-    const h8 hi = *(const h8 *)p, lo = *(const h8 *)(p + 16);
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = (float)hi[i] + (float)lo[i];
-}
-
 // X' = the packed transpose of G / |G| (G itself, row by row, when it is tall), [np][mp]; one 64 x 64 tile of G per workgroup
 template <class T> __global__ __launch_bounds__(256) void k_split(Ptrs p, Shape s, int parts, const double *sums, char *XT)
 {
@@ -141,7 +134,7 @@ template <class T> __global__ __launch_bounds__(256) void k_split(Ptrs p, Shape 
     }
 }
 
-// ---- packed products:  D = alpha * (A B') + beta * E + gamma * I,  A [M][K], B [N][K] packed
+// ---- packed products:  D' = alpha * (A B') + beta * E + gamma * I,  A [M][K], B [N][K] packed
 struct Gemm {
     const char *A, *B;
     size_t sA, sB;      // bytes from one matrix of the batch to the next
@@ -152,7 +145,7 @@ struct Gemm {
     float alpha, beta, gamma;
     const char *E;      // packed, same shape as D; or NULL
     size_t sE, sD;
-    char *D;            // packed result [M][N]; NULL: to p.out[], as G (D is its transpose, or itself when it is tall)
+    char *D;            // packed result, by columns: [N][M]; NULL: to p.out[] as G (columns: n, rows: m)
     int pitchD;
 };
 
@@ -215,19 +208,71 @@ __device__ __forceinline__ void tile_at(int i, const Gemm &a, int &ti, int &tj)
     }
 }
 
-// BM x BN results per workgroup of KS groups of 4 wavefronts (2 x 2); per stage and wavefront (BM/64) (BN/64) 2 x 3 matrix
+// Where a finished tile stands in LDS: [column][row], so that the four rows a lane has of a column are one write, with
+// rows exchanged in fours so that reads along the columns find all banks
+template <int BM> __device__ __forceinline__ int tile_place(int r, int c) { return c * (BM + 4) + (r ^ (c >> 3 & 7) << 2); }
+
+// A finished tile from LDS to its place, every write a whole group of 8.  The result is stored by columns (D is [N][M]);
+// symmetric ones also where the mirror image belongs.
+template <int BM, int BN, int THREADS, class T>
+__device__ __forceinline__ void store_tile(float *t, const Gemm &a, const Ptrs &p, const Shape &s, int b, int ti, int tj)
+{
+    const int row0 = ti * BM, col0 = tj * BN; // rows: m, columns: n
+    if (!a.D) {
+        T *out = (T *)p.out[b];
+        for (int e = threadIdx.x; e < BM * BN; e += THREADS) {
+            if (s.tall) {
+                const int c = e / BM, r = e % BM;
+                if (row0 + r < s.m && col0 + c < s.n) put(out + (size_t)(col0 + c) * s.ld_out + row0 + r, t[tile_place<BM>(r, c)]);
+            } else { // 4 rows of 16 columns per wavefront: all banks
+                const int c = (e >> 6) % (BN / 16) * 16 + (e & 15), r = (e >> 6) / (BN / 16) * 4 + (e >> 4 & 3);
+                if (row0 + r < s.m && col0 + c < s.n) put(out + (size_t)(row0 + r) * s.ld_out + col0 + c, t[tile_place<BM>(r, c)]);
+            }
+        }
+        return;
+    }
+    char *D = a.D + b * a.sD;
+    for (int e = threadIdx.x; e < BM * BN / 8; e += THREADS) {
+        const int c = e / (BM / 8), r = e % (BM / 8) * 8;
+        float4 *lo4 = (float4 *)(t + tile_place<BM>(r, c)), *hi4 = (float4 *)(t + tile_place<BM>(r + 4, c));
+        float4 x = *lo4, y = *hi4;
+        float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        const size_t at = (size_t)(col0 + c) * a.pitchD + (size_t)(row0 + r) * 4;
+        if (a.E) {
+            const h8 hi = *(const h8 *)(a.E + b * a.sE + at), lo = *(const h8 *)(a.E + b * a.sE + at + 16);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                v[i] = fmaf(a.beta, (float)hi[i] + (float)lo[i], v[i]) + (col0 + c == row0 + r + i ? a.gamma : 0.f);
+            *lo4 = make_float4(v[0], v[1], v[2], v[3]);
+            *hi4 = make_float4(v[4], v[5], v[6], v[7]);
+        }
+        pack8(D + at, v);
+    }
+    if (!a.symmetric || ti == tj) return;
+    __syncthreads();
+    for (int e = threadIdx.x; e < BM * BN / 8; e += THREADS) {
+        const int r = e / (BN / 8), c = e % (BN / 8) * 8;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = t[tile_place<BM>(r, c + i)];
+        pack8(D + (size_t)(row0 + r) * a.pitchD + (size_t)(col0 + c) * 4, v);
+    }
+}
+
+// BM x BN results per workgroup of 4 wavefronts (2 x 2); per stage and wavefront (BM/64) (BN/64) 2 x 3 matrix
 // instructions 32x32x16 on (BM/64 + BN/64) 4 LDS reads.  Two stages in LDS: the next one loads while this one is used.
-// The groups take every KS-th stage of K and add up at the end: more wavefronts per CU where tiles are few.
+// KS groups of 4 wavefronts take every KS-th stage of K, each with stages of its own, and add up at the end: where tiles
+// are few a CU needs more loads in flight (what one asks for arrives after 2100 cycles).  Measured with one group /
+// four: 256 x 2304, one matrix 225 / 174 us, 4 x 512 x 512 191 / 153 us.  (Every wavefront on its own, a whole tile each,
+// with four pieces of K in flight: 200 and 173 us.)
 // TURN: A and B are given as [K][M] and [K][N] (the Gram matrix from X'), and the LDS reads transpose.
 template <int BM, int BN, int KS, bool TURN, class T>
 __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs p, Shape s)
 {
     constexpr int FM = BM / 64, FN = BN / 64; // 32 x 32 blocks of a wavefront
     constexpr int STAGE = (BM + BN) * 128;
-    constexpr int LT = BN + 1;
-    constexpr int TILE = BM * LT * 4;
-    constexpr int THREADS = 256 * KS;
-    __shared__ __align__(16) char lds_all[2 * KS * STAGE > TILE ? 2 * KS * STAGE : TILE];
+    constexpr int TILE = BN * (BM + 4) * 4;
+    __shared__ __align__(16) char lds_all[KS * (2 * STAGE > TILE ? 2 * STAGE : TILE)];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
     const int group = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     char *lds = lds_all + group * 2 * STAGE;
@@ -337,66 +382,34 @@ __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs
                 }
         }
     }
-    // the tile through LDS, so that every write is a whole group of 8 whichever way the result is stored
     __syncthreads();
-    float *t = (float *)lds_all;
+    float *t = (float *)lds_all, *part = (float *)(lds_all + group * TILE);
 #pragma unroll
-    for (int g = KS - 1; g >= 0; g--) { // the groups one after the other: a fixed order
-        if (group == g) {
+    for (int i = 0; i < FM; i++)
 #pragma unroll
-            for (int i = 0; i < FM; i++)
+        for (int j = 0; j < FN; j++)
 #pragma unroll
-                for (int j = 0; j < FN; j++)
+            for (int e = 0; e < 16; e += 4) {
+                float v[4];
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const int r = wm + i * 32 + (e >> 2) * 8 + half * 4 + (e & 3), c = wn + j * 32 + lr;
-                        const float v = (acc[i][j][e] + low[i][j][e]) * a.alpha;
-                        t[r * LT + c] = g == KS - 1 ? v : v + t[r * LT + c];
-                    }
+                for (int q = 0; q < 4; q++) v[q] = (acc[i][j][e + q] + low[i][j][e + q]) * a.alpha;
+                *(float4 *)(part + tile_place<BM>(wm + i * 32 + e * 2 + half * 4, wn + j * 32 + lr)) = make_float4(v[0], v[1], v[2], v[3]);
+            }
+    __syncthreads();
+    if (KS > 1) { // the groups' sums in their order
+        for (int e = threadIdx.x; e < BM * BN / 4; e += 256 * KS) {
+            const int at = tile_place<BM>(e % (BM / 4) * 4, e / (BM / 4));
+            float4 v = *(float4 *)(t + at);
+#pragma unroll
+            for (int g = 1; g < KS; g++) {
+                const float4 o = *(const float4 *)(t + g * (TILE / 4) + at);
+                v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+            }
+            *(float4 *)(t + at) = v;
         }
         __syncthreads();
     }
-    const int row0 = ti * BM, col0 = tj * BN;
-    if (!a.D) { // rows of the result: n, columns: m
-        T *out = (T *)p.out[b];
-        for (int e = threadIdx.x; e < BM * BN; e += THREADS) {
-            if (s.tall) {
-                const int r = e / BN, c = e % BN;
-                if (row0 + r < s.n && col0 + c < s.m) put(out + (size_t)(row0 + r) * s.ld_out + col0 + c, t[r * LT + c]);
-            } else {
-                const int c = e / BM, r = e % BM;
-                if (row0 + r < s.n && col0 + c < s.m) put(out + (size_t)(col0 + c) * s.ld_out + row0 + r, t[r * LT + c]);
-            }
-        }
-        return;
-    }
-    char *D = a.D + b * a.sD;
-    for (int e = threadIdx.x; e < BM * BN / 8; e += THREADS) {
-        const int r = e / (BN / 8), c = e % (BN / 8) * 8;
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = t[r * LT + c + i];
-        const size_t at = (size_t)(row0 + r) * a.pitchD + (size_t)(col0 + c) * 4;
-        if (a.E) {
-            float w[8];
-            unpack8(a.E + b * a.sE + at, w);
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                v[i] = fmaf(a.beta, w[i], v[i]) + (row0 + r == col0 + c + i ? a.gamma : 0.f);
-                t[r * LT + c + i] = v[i];
-            }
-        }
-        pack8(D + at, v);
-    }
-    if (!a.symmetric || ti == tj) return;
-    __syncthreads();
-    for (int e = threadIdx.x; e < BM * BN / 8; e += THREADS) {
-        const int c = e / (BM / 8), r = e % (BM / 8) * 8;
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = t[(r + i) * LT + c];
-        pack8(D + (size_t)(col0 + c) * a.pitchD + (size_t)(row0 + r) * 4, v);
-    }
+    store_tile<BM, BN, 256 * KS, T>(t, a, p, s, b, ti, tj);
 }
 
 // ---------------------------------------------------------------- small matrices: all steps in one launch
@@ -824,9 +837,9 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
         }
         const char *total = k == 1 ? W : Q;
         left -= k;
-        Gemm g = {}; // X' <- X' Q
-        g.A = XT; g.B = total;
-        g.sA = pl.x; g.sB = pl.mm;
+        Gemm g = {}; // X <- Q X, by columns
+        g.A = total; g.B = XT;
+        g.sA = pl.mm; g.sB = pl.x;
         g.pitchA = g.pitchB = pm;
         g.K = s.mp;
         g.alpha = two((left ? EXP_X : 0) - EXP_Q - EXP_X);
@@ -835,7 +848,7 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
             g.D = YT;
             g.pitchD = pm;
         }
-        gemm(g, s.np, s.mp, false, batch, dtype, p, s, st);
+        gemm(g, s.mp, s.np, false, batch, dtype, p, s, st);
         char *t = XT;
         XT = YT;
         YT = t;

@@ -945,7 +945,8 @@ int az_policy_loss(int n, int actions, const void *d_logits, int dtype, long lon
 {
     const Rows a = {d_logits, ld, d_board, d_legal, ld_legal, n, actions};
     if (!rows_ok(a, dtype) || n < 1) return AZ_ERR_ARG;
-    if (!d_logits || !d_value || !d_pi || !d_r || !d_work || (only_if_scaled && !d_scale) || (d_parts && !d_loss)) return AZ_ERR_ARG;
+    if (!d_work && (d_loss || actions > SHORT_MAX)) return AZ_ERR_ARG;
+    if (!d_logits || !d_value || !d_pi || !d_r || (only_if_scaled && !d_scale) || (d_parts && !d_loss)) return AZ_ERR_ARG;
     Loss o = {d_value, value_f32, d_pi, d_r, 1.f / (float)n, d_scale, only_if_scaled, d_loss ? (double *)d_work : nullptr, d_dlogits, d_dvalue};
     const dim3 block(64 * WAVES);
     const hipStream_t st = (hipStream_t)stream;

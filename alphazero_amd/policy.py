@@ -18,6 +18,7 @@ from . import engine as _E
 
 MAX_MOVES, MAX_TOP = 64, 32  # AZ_POLICY_MAX_MOVES, AZ_POLICY_MAX_TOP
 MAX_ACTIONS = 1 << 24
+SHORT_MAX = 1024  # rows up to here are held in registers
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # AZ_F32, AZ_BF16, AZ_F16
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
@@ -113,6 +114,15 @@ def _rows(logits, board, legal):
     return logits, board, legal, (n, actions, logits.data_ptr(), kind, ld, at_board, at_legal, ld_legal)
 
 
+def _saved(rows, logits, board, legal):
+    """Tensors that come back from autograd and the entry points' leading arguments, made again where a saved-tensor hook
+    has moved a tensor."""
+    if logits.data_ptr() == rows[2] and _ptr(board) == rows[5] and _ptr(legal) == rows[6] and \
+            (rows[0] <= 1 or (logits.stride(0) == rows[4] and (legal is None or legal.stride(0) == rows[7]))):
+        return logits, board, legal, rows
+    return _rows(logits, board, legal)
+
+
 def _score_forward(logits, moves, board, legal, top, rows, device, keep):
     n, actions = rows[:2]
     new = logits.new_empty
@@ -134,7 +144,7 @@ class _ScoreFunction(torch.autograd.Function):
     def forward(ctx, logits, moves, board, legal, top, rows, device):
         logp, entropy, top_moves, top_logp, stats, bits = _score_forward(logits, moves, board, legal, top, rows, device, True)
         ctx.set_materialize_grads(False)
-        ctx.device = device
+        ctx.rows, ctx.device = rows, device
         if top:
             ctx.mark_non_differentiable(top_moves, top_logp)
         ctx.save_for_backward(logits, moves, board, legal, entropy, stats, bits)
@@ -144,7 +154,7 @@ class _ScoreFunction(torch.autograd.Function):
     def backward(ctx, g_logp, g_entropy, _moves, _logp):
         _once()
         logits, moves, board, legal, entropy, stats, bits = ctx.saved_tensors
-        logits, board, legal, rows = _rows(logits, board, legal)  # (a saved-tensor hook may have moved them)
+        logits, board, legal, rows = _saved(ctx.rows, logits, board, legal)
         if g_logp is None and g_entropy is None:
             return (None,) * 7
         d = logits.new_empty(logits.shape)
@@ -187,9 +197,9 @@ def score(logits, moves=None, *, board=None, legal=None, top=0):
 
 
 def _loss_call(rows, device, value, pi, r, scale, only_if_scaled, total, parts, d_logits, d_value):
-    work = pi.new_empty((_loss_work(rows[0], rows[1]),), dtype=torch.uint8)
+    work = None if total is None and rows[1] <= SHORT_MAX else pi.new_empty((_loss_work(rows[0], rows[1]),), dtype=torch.uint8)
     _call("az_policy_loss", device, *rows, value.data_ptr(), int(value.dtype == torch.float32), pi.data_ptr(), r.data_ptr(),
-          _ptr(scale), only_if_scaled, _ptr(total), _ptr(parts), _ptr(d_logits), _ptr(d_value), work.data_ptr())
+          _ptr(scale), only_if_scaled, _ptr(total), _ptr(parts), _ptr(d_logits), _ptr(d_value), _ptr(work))
 
 
 class _LossFunction(torch.autograd.Function):
@@ -207,7 +217,7 @@ class _LossFunction(torch.autograd.Function):
         _loss_call(rows, device, value, pi, r, None, 0, total, parts, d_logits, d_value)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, value, pi, r, board, legal)
-        ctx.device, ctx.ready = device, (d_logits, d_value)
+        ctx.rows, ctx.device, ctx.ready = rows, device, (d_logits, d_value)
         if want_parts:
             ctx.mark_non_differentiable(parts)
         return total, parts
@@ -216,7 +226,7 @@ class _LossFunction(torch.autograd.Function):
     def backward(ctx, g, _parts):
         _once()
         logits, value, pi, r, board, legal = ctx.saved_tensors
-        logits, board, legal, rows = _rows(logits, board, legal)  # (a saved-tensor hook may have moved them)
+        logits, board, legal, rows = _saved(ctx.rows, logits, board, legal)
         ready, ctx.ready = ctx.ready, None  # given away once: a second backward pass computes its own
         if ready is None:
             need_l, need_v = ctx.needs_input_grad[:2]

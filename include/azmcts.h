@@ -471,7 +471,7 @@ int az_policy_score_grad(int n, int actions, const void *d_logits, int dtype, lo
  *   d_dlogits [n][actions] (type of the logits), d_dvalue [n] (type of the values): gradients of the total times
  *   *d_scale (device float; NULL: 1); either may be NULL.  only_if_scaled: do nothing when *d_scale is 1 (the buffers
  *   hold the gradients of an earlier call with the same inputs and no scale).
- * d_work: az_policy_loss_work(n, actions) bytes, used by this call only. */
+ * d_work: az_policy_loss_work(n, actions) bytes, used by this call only (may be NULL up to 1024 actions when d_loss is). */
 long long az_policy_loss_work(int n, int actions);
 int az_policy_loss(int n, int actions, const void *d_logits, int dtype, long long ld, const float *d_board,
                    const unsigned char *d_legal, long long ld_legal, const void *d_value, int value_f32, const float *d_pi,
