@@ -47,37 +47,51 @@ __device__ __forceinline__ void put(f16_t *p, size_t i, float v) { p[i].h = (_Fl
 // the value falls as e^d: what reaches a sum of probabilities stays below 2^-22
 __device__ __forceinline__ float exp_neg(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }
 
-template <int CTRL> __device__ __forceinline__ float dpp(float old, float v)
+// the value of another lane of the wavefront (0 where the pattern names none), as an operand of the instruction using it
+template <int CTRL> __device__ __forceinline__ uint32_t dpp(uint32_t v)
 {
-    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL, 0xf, 0xf, false));
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
 }
+template <int CTRL> __device__ __forceinline__ float dpp(float v) { return __uint_as_float(dpp<CTRL>(__float_as_uint(v))); }
 __device__ __forceinline__ float lane_of(float v, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); }
 __device__ __forceinline__ float wave_sum(float v)
 {
-    v += dpp<0x111>(0.f, v); // row_shr 1, 2, 4, 8: lane 15 of each row of 16 holds the row's sum
-    v += dpp<0x112>(0.f, v);
-    v += dpp<0x114>(0.f, v);
-    v += dpp<0x118>(0.f, v);
-    v += dpp<0x142>(0.f, v); // lane 15 / 47 to the next row, lane 31 to the upper half: lane 63 holds all
-    v += dpp<0x143>(0.f, v);
+    v += dpp<0x111>(v); // row_shr 1, 2, 4, 8: lane 15 of each row of 16 holds the row's sum
+    v += dpp<0x112>(v);
+    v += dpp<0x114>(v);
+    v += dpp<0x118>(v);
+    v += dpp<0x142>(v); // lane 15 / 47 to the next row, lane 31 to the upper half: lane 63 holds all
+    v += dpp<0x143>(v);
     return lane_of(v, 63);
 }
-__device__ __forceinline__ float wave_max(float v) // NaN is ignored
+// unsigned numbers in the order of the floats (0 is below all of them; NaN counts as -inf, -0 as 0)
+__device__ __forceinline__ uint32_t order_of(float v)
 {
-    v = fmaxf(v, dpp<0x111>(NINF, v));
-    v = fmaxf(v, dpp<0x112>(NINF, v));
-    v = fmaxf(v, dpp<0x114>(NINF, v));
-    v = fmaxf(v, dpp<0x118>(NINF, v));
-    v = fmaxf(v, dpp<0x142>(NINF, v));
-    v = fmaxf(v, dpp<0x143>(NINF, v));
-    return lane_of(v, 63);
+    const uint32_t b = __float_as_uint(fmaxf(v, NINF) + 0.f);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ float float_of(uint32_t k) { return __uint_as_float(k ^ ((uint32_t)(~(int32_t)k >> 31) | 0x80000000u)); }
+__device__ __forceinline__ uint32_t wave_max(uint32_t v)
+{
+    v = max(v, dpp<0x111>(v));
+    v = max(v, dpp<0x112>(v));
+    v = max(v, dpp<0x114>(v));
+    v = max(v, dpp<0x118>(v));
+    v = max(v, dpp<0x142>(v));
+    v = max(v, dpp<0x143>(v));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ float wave_max(float v) { return float_of(wave_max(order_of(v))); } // NaN is ignored
 __device__ __forceinline__ double wave_sum(double v)
 {
 #pragma unroll
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
+
+// the wavefront's number, known to be the same in all lanes: what depends on it alone (a row's address) costs no vector
+// instruction
+__device__ __forceinline__ int wave_of() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 struct Rows {
     const void *x;          // logits [n][ld]
@@ -97,12 +111,19 @@ __device__ __forceinline__ bool legal_at(const Rows &a, size_t row, int j)
     return a.legal ? a.legal[row * (size_t)a.ldl + j] != 0 : true;
 }
 
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(bf16_t v) { return __uint_as_float((uint32_t)v.u << 16); }
+__device__ __forceinline__ float as_float(f16_t v) { return (float)v.h; }
+
 // The row's cells of this lane, -inf where the mask or the row's end leaves nothing (a select: what stands in a masked
-// place is never computed with).  All loads are issued before the first use.
+// place is never computed with).  The logits are asked for before the mask, so that the row waits for memory once.
 template <class T, int R> __device__ __forceinline__ void load_row(const Rows &a, size_t row, int lane, float (&x)[R])
 {
     const T *p = (const T *)a.x + row * (size_t)a.ld;
+    T raw[R];
     bool ok[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) raw[r] = p[min(r * 64 + lane, a.A - 1)];
     if (a.board) {
         const float *b = a.board + row * 2 * (size_t)a.A;
         float b0[R], b1[R];
@@ -113,8 +134,6 @@ template <class T, int R> __device__ __forceinline__ void load_row(const Rows &a
             b1[r] = b[a.A + j];
         }
 #pragma unroll
-        for (int r = 0; r < R; r++) x[r] = get(p, min(r * 64 + lane, a.A - 1));
-#pragma unroll
         for (int r = 0; r < R; r++) ok[r] = b0[r] == 0.f && b1[r] == 0.f;
     } else if (a.legal) {
         const uint8_t *q = a.legal + row * (size_t)a.ldl;
@@ -122,17 +141,13 @@ template <class T, int R> __device__ __forceinline__ void load_row(const Rows &a
 #pragma unroll
         for (int r = 0; r < R; r++) l[r] = q[min(r * 64 + lane, a.A - 1)];
 #pragma unroll
-        for (int r = 0; r < R; r++) x[r] = get(p, min(r * 64 + lane, a.A - 1));
-#pragma unroll
         for (int r = 0; r < R; r++) ok[r] = l[r] != 0;
     } else {
-#pragma unroll
-        for (int r = 0; r < R; r++) x[r] = get(p, min(r * 64 + lane, a.A - 1));
 #pragma unroll
         for (int r = 0; r < R; r++) ok[r] = true;
     }
 #pragma unroll
-    for (int r = 0; r < R; r++) x[r] = ok[r] && r * 64 + lane < a.A ? x[r] : NINF;
+    for (int r = 0; r < R; r++) x[r] = ok[r] && r * 64 + lane < a.A ? as_float(raw[r]) : NINF;
 }
 
 struct Stats { float M, logS, H; bool live; };
@@ -168,15 +183,15 @@ struct Best { float v; int i; };
 __device__ __forceinline__ void best_insert(Best &b, float v, int i, int lane) // v, i uniform; equal values stay in front
 {
     const int pos = __popcll(__ballot(b.v >= v));
-    const float uv = dpp<0x138>(NINF, b.v); // from the lane below
-    const int ui = __builtin_amdgcn_update_dpp(-1, b.i, 0x138, 0xf, 0xf, false);
+    const float uv = dpp<0x138>(b.v); // from the lane below
+    const int ui = (int)dpp<0x138>((uint32_t)b.i);
     b.v = lane < pos ? b.v : lane == pos ? v : uv;
     b.i = lane < pos ? b.i : lane == pos ? i : ui;
 }
 
 // The cells of a step, whose indices (first + 64 r + lane) all come after those already listed.  Of many candidates only
-// those not below the k-th largest of the 64 lane maxima can be among the k best, few more than k as a rule; those are
-// put into the list one by one, in the order of their indices.
+// those not below the k-th largest of the 64 lane maxima can be among the k best, few more than k as a rule (the bound is
+// found to 16 bits, from below); those are put into the list one by one, in the order of their indices.
 template <int R> __device__ __forceinline__ void best_offer(Best &b, const float (&x)[R], int first, int k, int lane)
 {
     float limit = lane_of(b.v, k - 1);
@@ -187,12 +202,12 @@ template <int R> __device__ __forceinline__ void best_offer(Best &b, const float
     if (!some) return;
     float least = NINF;
     if (__popcll(some) > k) {
-        float v = top > limit ? top : NINF;
-        for (int i = 1; i < k; i++) {
-            const unsigned long long at = __ballot(v == wave_max(v));
-            if (lane == __ffsll(at) - 1) v = NINF;
-        }
-        least = wave_max(v);
+        const uint32_t key = order_of(top);
+        uint32_t bound = 0;
+        for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1)
+            if (__popcll(__ballot(key >= (bound | bit))) >= k) bound |= bit;
+        least = float_of(bound);
+        if (!(least > NINF)) least = NINF; // (a bound below every number is no number)
     }
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -228,8 +243,9 @@ template <class T, int R> __global__ __launch_bounds__(64 * WAVES) void k_score(
 {
     const int lane = threadIdx.x & 63;
     const int words = (a.A + 63) / 64;
-    for (long long row = (long long)blockIdx.x * WAVES + (threadIdx.x >> 6); row < a.n; row += (long long)gridDim.x * WAVES) {
+    for (long long row = (long long)blockIdx.x * WAVES + wave_of(); row < a.n; row += (long long)gridDim.x * WAVES) {
         float x[R];
+        const long long mv = lane < o.m ? move_at(o.moves, o.move_bytes, (size_t)row * o.m + lane) : -1;
         load_row<T, R>(a, row, lane, x);
         if (o.bits) {
 #pragma unroll
@@ -247,7 +263,6 @@ template <class T, int R> __global__ __launch_bounds__(64 * WAVES) void k_score(
             }
         }
         if (o.m) {
-            const long long mv = lane < o.m ? move_at(o.moves, o.move_bytes, (size_t)row * o.m + lane) : -1;
             const int at = mv >= 0 && mv < a.A ? (int)mv : -1;
             float v = NINF;
 #pragma unroll
@@ -313,8 +328,15 @@ template <class T, int R> __global__ __launch_bounds__(64 * WAVES) void k_score_
 {
     const int lane = threadIdx.x & 63;
     const int words = (a.A + 63) / 64;
-    for (long long row = (long long)blockIdx.x * WAVES + (threadIdx.x >> 6); row < a.n; row += (long long)gridDim.x * WAVES) {
+    for (long long row = (long long)blockIdx.x * WAVES + wave_of(); row < a.n; row += (long long)gridDim.x * WAVES) {
+        // everything the row needs is asked for before anything is waited for
         float x[R];
+        const bool given = o.m && o.g_logp;
+        const long long mv = given && lane < o.m ? move_at(o.moves, o.move_bytes, (size_t)row * o.m + lane) : -1;
+        const float up = given && lane < o.m ? o.g_logp[(size_t)row * o.m + lane] : 0.f;
+        const float M = o.stats[2 * row], logS = o.stats[2 * row + 1];
+        const float gH = o.g_entropy ? o.g_entropy[row] : 0.f;
+        const float H = o.g_entropy ? o.entropy[row] : 0.f;
         if (o.bits) {
             Rows plain = a;
             plain.board = nullptr;
@@ -328,12 +350,10 @@ template <class T, int R> __global__ __launch_bounds__(64 * WAVES) void k_score_
         } else {
             load_row<T, R>(a, row, lane, x);
         }
-        const float M = o.stats[2 * row], logS = o.stats[2 * row + 1];
         const bool live = !(M == NINF);
         float g = 0.f;
         int at = -1;
-        if (o.m && o.g_logp) {
-            const long long mv = lane < o.m ? move_at(o.moves, o.move_bytes, (size_t)row * o.m + lane) : -1;
+        if (given) {
             at = mv >= 0 && mv < a.A ? (int)mv : -1;
             float v = NINF;
 #pragma unroll
@@ -342,11 +362,9 @@ template <class T, int R> __global__ __launch_bounds__(64 * WAVES) void k_score_
                 v = (at >> 6) == r ? c : v;
             }
             at = v == NINF ? -1 : at;
-            g = at >= 0 ? o.g_logp[(size_t)row * o.m + lane] : 0.f;
+            g = at >= 0 ? up : 0.f;
         }
-        const float G = o.m && o.g_logp ? wave_sum(g) : 0.f;
-        const float gH = o.g_entropy ? o.g_entropy[row] : 0.f;
-        const float H = o.g_entropy ? o.entropy[row] : 0.f;
+        const float G = given ? wave_sum(g) : 0.f;
         float d[R];
 #pragma unroll
         for (int r = 0; r < R; r++) {
@@ -355,7 +373,7 @@ template <class T, int R> __global__ __launch_bounds__(64 * WAVES) void k_score_
             const float ent = p == 0.f ? 0.f : gH * p * (lp + H);
             d[r] = x[r] == NINF || !live ? 0.f : -p * G - ent;
         }
-        if (o.m && o.g_logp && live) {
+        if (given && live) {
             for (int i = 0; i < o.m; i++) {
                 const int j = __builtin_amdgcn_readlane(at, i);
                 const float gi = lane_of(g, i);
@@ -433,7 +451,7 @@ template <class T, int R> __global__ __launch_bounds__(64 * WAVES) void k_loss(R
     const int lane = threadIdx.x & 63;
     double sum = 0.;
     const float f = o.inv_n * scale;
-    for (long long row = (long long)blockIdx.x * WAVES + (threadIdx.x >> 6); row < a.n; row += (long long)gridDim.x * WAVES) {
+    for (long long row = (long long)blockIdx.x * WAVES + wave_of(); row < a.n; row += (long long)gridDim.x * WAVES) {
         const float *pi = o.pi + (size_t)row * a.A;
         float x[R], q[R];
 #pragma unroll
@@ -521,7 +539,7 @@ template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_parts(Ro
 {
     if (o.unless_one && *o.unless_one == 1.f) return;
     const int lane = threadIdx.x & 63;
-    const long long unit = (long long)blockIdx.x * WAVES + (threadIdx.x >> 6);
+    const long long unit = (long long)blockIdx.x * WAVES + wave_of();
     if (unit >= (long long)a.n * c.count) return;
     const long long row = unit / c.count;
     const int chunk = (int)(unit - row * c.count);
@@ -605,19 +623,33 @@ __device__ __forceinline__ Part join_parts(const Part *part, int count, int lane
     return Part{M, wave_sum(S), wave_sum(U), wave_sum(W), wave_sum(E), wave_sum(X)};
 }
 
-// one wavefront per row: outputs of az_policy_score from the chunks' numbers and lists.  The lists are merged in LDS: a
+// one workgroup per row: outputs of az_policy_score from the chunks' numbers and lists.  The lists are merged in LDS: a
 // lane holds the heads of every 64th list, each round takes the largest head (of equal ones the lowest index)
-template <class T> __global__ __launch_bounds__(64) void k_long_score(Rows a, Chunks c, LongOut w, ScoreOut o)
+template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_score(Rows a, Chunks c, LongOut w, ScoreOut o)
 {
     extern __shared__ float s_list[]; // [chunks][top] values, then indices
     const int lane = threadIdx.x;
     const long long row = blockIdx.x;
     const int cells = c.count * o.top;
     int *s_index = (int *)(s_list + cells);
-    for (int i = lane; i < cells; i += 64) {
-        s_list[i] = w.list_v[(size_t)row * cells + i];
-        s_index[i] = w.list_i[(size_t)row * cells + i];
+    for (int i = lane; i < cells; i += 64 * WAVES * 4) { // four loads in flight per thread
+        float v[4];
+        int n[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const size_t at = (size_t)row * cells + min(i + q * 64 * WAVES, cells - 1);
+            v[q] = w.list_v[at];
+            n[q] = w.list_i[at];
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            if (i + q * 64 * WAVES < cells) {
+                s_list[i + q * 64 * WAVES] = v[q];
+                s_index[i + q * 64 * WAVES] = n[q];
+            }
     }
+    __syncthreads();
+    if (lane >= 64) return; // the first wavefront does the rest
     const Part t = join_parts(w.part + (size_t)row * c.count, c.count, lane);
     const bool live = t.S != 0.f;
     const float logS = live ? logf(t.S) : 0.f;
@@ -640,7 +672,6 @@ template <class T> __global__ __launch_bounds__(64) void k_long_score(Rows a, Ch
         o.logp[(size_t)row * o.m + lane] = r;
     }
     if (!o.top) return;
-    __syncthreads();
     constexpr int HEADS = MAX_CHUNKS / 64;
     float head[HEADS];
     int next[HEADS]; // where the head's successor stands
@@ -695,7 +726,7 @@ template <class T> __global__ __launch_bounds__(64) void k_long_score(Rows a, Ch
 template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_score_grad(Rows a, Chunks c, ScoreGrad o)
 {
     const int lane = threadIdx.x & 63;
-    const long long unit = (long long)blockIdx.x * WAVES + (threadIdx.x >> 6);
+    const long long unit = (long long)blockIdx.x * WAVES + wave_of();
     if (unit >= (long long)a.n * c.count) return;
     const long long row = unit / c.count;
     const int chunk = (int)(unit - row * c.count);
@@ -754,7 +785,7 @@ template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_loss(Row
     const float f = o.inv_n * scale;
     double sum = 0.;
     const long long units = (long long)a.n * c.count;
-    for (long long unit = (long long)blockIdx.x * WAVES + (threadIdx.x >> 6); unit < units; unit += (long long)gridDim.x * WAVES) {
+    for (long long unit = (long long)blockIdx.x * WAVES + wave_of(); unit < units; unit += (long long)gridDim.x * WAVES) {
         const long long row = unit / c.count;
         const int chunk = (int)(unit - row * c.count);
         const int begin = chunk * c.len, end = min(a.A, begin + c.len);
@@ -897,7 +928,7 @@ int az_policy_score(int n, int actions, const void *d_logits, int dtype, long lo
     by_type(dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
         hipLaunchKernelGGL((k_long_parts<T>), dim3((unsigned)((units + WAVES - 1) / WAVES)), block, 0, st, a, c, w);
-        hipLaunchKernelGGL((k_long_score<T>), dim3(n), dim3(64), (size_t)c.count * top * 8, st, a, c, w, o);
+        hipLaunchKernelGGL((k_long_score<T>), dim3(n), block, (size_t)c.count * top * 8, st, a, c, w, o);
     });
     return launch_ok();
 }
