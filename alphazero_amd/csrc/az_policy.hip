@@ -11,6 +11,7 @@
 //   longer rows                   one wavefront per chunk of a row; partial (M, S, U) per chunk in a workspace,
 //                                 joined by the launch that needs them.
 #include <hip/hip_runtime.h>
+#include <float.h>
 #include <math.h>
 #include <stdint.h>
 #include <type_traits>
@@ -152,26 +153,35 @@ template <class T, int R> __device__ __forceinline__ void load_row(const Rows &a
 
 struct Stats { float M, logS, H; bool live; };
 
+// e^(x - M) and x - M of a cell, 0 and a finite number for a cell of -inf.  M must not be -inf.
+__device__ __forceinline__ float term(float x, float M, float &d)
+{
+    const float t = x - M;
+    d = fmaxf(t, -FLT_MAX); // (what multiplies it is 0 there)
+    return exp_neg(t);
+}
+
 // M, log S and the entropy of a row in registers
 template <int R> __device__ __forceinline__ Stats row_stats(const float (&x)[R])
 {
     float m = x[0];
 #pragma unroll
     for (int r = 1; r < R; r++) m = fmaxf(m, x[r]);
-    const float M = wave_max(m);
+    Stats t;
+    t.M = wave_max(m);
+    const float M = t.M == NINF ? 0.f : t.M;
     float s = 0.f, u = 0.f;
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        const float d = x[r] - M;
-        const float e = x[r] == NINF ? 0.f : exp_neg(d);
+        float d;
+        const float e = term(x[r], M, d);
         s += e;
-        u += e == 0.f ? 0.f : e * d;
+        u = fmaf(e, d, u);
     }
     s = wave_sum(s);
     u = wave_sum(u);
-    Stats t;
     t.live = s != 0.f; // (a NaN cell makes s NaN: the row is live and all of it is NaN)
-    t.M = t.live && M == NINF ? NAN : M; // (legal cells that are all NaN)
+    t.M = t.live && t.M == NINF ? NAN : t.M; // (legal cells that are all NaN)
     t.logS = t.live ? logf(s) : 0.f;
     t.H = t.live ? t.logS - u / s : 0.f;
     return t;
@@ -247,12 +257,14 @@ template <class T, int R> __global__ __launch_bounds__(64 * WAVES) void k_score(
         float x[R];
         const long long mv = lane < o.m ? move_at(o.moves, o.move_bytes, (size_t)row * o.m + lane) : -1;
         load_row<T, R>(a, row, lane, x);
-        if (o.bits) {
+        if (o.bits) { // lane r stores the mask of register r
+            unsigned long long mine = 0;
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 const unsigned long long w = __ballot(x[r] != NINF);
-                if (lane == 0 && r < words) o.bits[(size_t)row * words + r] = w;
+                mine = lane == r ? w : mine;
             }
+            if (lane < words) o.bits[(size_t)row * words + lane] = mine;
         }
         const Stats t = row_stats<R>(x);
         if (lane == 0) {
@@ -400,10 +412,8 @@ struct Loss {
     void *dx, *dv;          // [n][A], [n], or NULL
 };
 
-__device__ __forceinline__ float policy_term(float pi, float lp)
-{
-    return pi == 0.f ? 0.f : pi * (__logf(pi) - lp); // a negative pi gives NaN
-}
+// log pi, finite for 0 (which multiplies it); NaN for a negative one
+__device__ __forceinline__ float log_of(float pi) { return pi == 0.f ? 0.f : __logf(pi); }
 
 // sums of a workgroup's wavefronts in wavefront order
 __device__ __forceinline__ void block_part(double p, double v, double *out)
@@ -460,24 +470,25 @@ template <class T, int R> __global__ __launch_bounds__(64 * WAVES) void k_loss(R
         float m = x[0];
 #pragma unroll
         for (int r = 1; r < R; r++) m = fmaxf(m, x[r]);
-        const float M = wave_max(m);
-        float s = 0.f, w = 0.f, e[R];
+        m = wave_max(m);
+        const float M = m == NINF ? 0.f : m;
+        float s = 0.f, w = 0.f, l = 0.f, e[R];
 #pragma unroll
         for (int r = 0; r < R; r++) {
             q[r] = x[r] == NINF ? 0.f : q[r]; // masked places (and cells past the row's end) hold no target
-            e[r] = x[r] == NINF ? 0.f : exp_neg(x[r] - M);
+            float d;
+            e[r] = term(x[r], M, d);
             s += e[r];
             w += q[r];
+            l += q[r] * (log_of(q[r]) - d);
         }
         s = wave_sum(s);
         w = wave_sum(w);
         const bool live = s != 0.f;
         if (o.part) {
-            const float logS = live ? logf(s) : 0.f;
-            float l = 0.f;
-#pragma unroll
-            for (int r = 0; r < R; r++) l += x[r] == NINF ? 0.f : policy_term(q[r], x[r] - M - logS);
-            sum += (double)l; // per lane; the lanes are added at the end
+            // sum pi log pi - sum pi (x - M), each lane its share; log S sum pi once
+            sum += (double)l;
+            if (lane == 0 && live) sum += (double)logf(s) * (double)w;
         }
         if (o.dx) {
             const float inv = live ? w / s : 0.f;
@@ -582,7 +593,7 @@ template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_parts(Ro
             if (pi) {
                 const float w = x[r] == NINF ? 0.f : q[r];
                 W += w;
-                E += w == 0.f ? 0.f : w * __logf(w);
+                E += w * log_of(w);
                 X += w == 0.f ? 0.f : w * d;
             }
         }
