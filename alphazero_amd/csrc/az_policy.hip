@@ -26,6 +26,10 @@ constexpr int MAX_ACTIONS = 1 << 24;
 constexpr int LONG_R = 16;               // cells per lane and step of a long row
 constexpr int LONG_STEP = 64 * LONG_R;
 constexpr int MAX_CHUNKS = 256;          // chunks per row
+// Workgroups of a launch over `units` wavefronts' work; more work per wavefront comes by striding over the grid.  Eight
+// workgroups per CU fill it (8 x 4 wavefronts), sixteen do better where memory is the bound: 262144 x 225 loss 165 -> 149 us
+// (4.3 -> 4.75 TB/s; the rows of a wavefront are then further apart than a multiple of the memory's interleaving).
+constexpr int GRID_MAX = 256 * 16;
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float NINF = -INFINITY;
 
@@ -416,9 +420,9 @@ struct Loss {
 __device__ __forceinline__ float log_of(float pi) { return pi == 0.f ? 0.f : __logf(pi); }
 
 // sums of a workgroup's wavefronts in wavefront order
-__device__ __forceinline__ void block_part(double p, double v, double *out)
+template <int W> __device__ __forceinline__ void block_part(double p, double v, double *out)
 {
-    __shared__ double s_p[WAVES], s_v[WAVES];
+    __shared__ double s_p[W], s_v[W];
     const int wave = threadIdx.x >> 6;
     p = wave_sum(p);
     v = wave_sum(v);
@@ -428,7 +432,7 @@ __device__ __forceinline__ void block_part(double p, double v, double *out)
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < WAVES; w++) {
+        for (int w = 1; w < W; w++) {
             p += s_p[w];
             v += s_v[w];
         }
@@ -499,19 +503,26 @@ template <class T, int R> __global__ __launch_bounds__(64 * WAVES) void k_loss(R
         }
     }
     const double v = value_part<T>(a, o, scale);
-    if (o.part) block_part(sum, v, o.part + 2 * (size_t)blockIdx.x);
+    if (o.part) block_part<WAVES>(sum, v, o.part + 2 * (size_t)blockIdx.x);
 }
 
 // the total, and the policy and value parts, from the workgroups' partial sums, added in a fixed order
-__global__ __launch_bounds__(64 * WAVES) void k_loss_join(const double *part, int blocks, double inv_n, float *loss, float *parts)
+constexpr int JOIN_WAVES = 16;
+__global__ __launch_bounds__(64 * JOIN_WAVES) void k_loss_join(const double *part, int blocks, double inv_n, float *loss, float *parts)
 {
+    constexpr int EACH = (GRID_MAX + 64 * JOIN_WAVES - 1) / (64 * JOIN_WAVES);
+    double2 in[EACH]; // (all in flight together)
+#pragma unroll
+    for (int k = 0; k < EACH; k++) in[k] = ((const double2 *)part)[min(k * 64 * JOIN_WAVES + (int)threadIdx.x, blocks - 1)];
     double p = 0., v = 0.;
-    for (int i = threadIdx.x; i < blocks; i += 64 * WAVES) {
-        p += part[2 * i];
-        v += part[2 * i + 1];
+#pragma unroll
+    for (int k = 0; k < EACH; k++) {
+        const bool mine = k * 64 * JOIN_WAVES + (int)threadIdx.x < blocks;
+        p += mine ? in[k].x : 0.;
+        v += mine ? in[k].y : 0.;
     }
     __shared__ double s_all[2];
-    block_part(p, v, s_all);
+    block_part<JOIN_WAVES>(p, v, s_all);
     if (threadIdx.x == 0) {
         loss[0] = (float)((s_all[0] + s_all[1]) * inv_n);
         if (parts) {
@@ -685,15 +696,15 @@ template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_score(Ro
     if (!o.top) return;
     constexpr int HEADS = MAX_CHUNKS / 64;
     float head[HEADS];
-    int next[HEADS]; // where the head's successor stands
+    int place[HEADS]; // where the head stands
 #pragma unroll
     for (int h = 0; h < HEADS; h++) {
         const int list = h * 64 + lane;
         head[h] = list < c.count ? s_list[list * o.top] : NINF;
-        next[h] = list * o.top + 1;
+        place[h] = list * o.top;
     }
     float mine_v = NINF;
-    int mine_i = -1;
+    int mine_at = -1;
     for (int k = 0; k < o.top; k++) {
         float v = head[0];
         int from = 0;
@@ -706,31 +717,30 @@ template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_score(Ro
         if (best == NINF) break;
         // of the lanes with this value the one whose list comes first holds the lowest index
         int list = v == best ? from * 64 + lane : 0x7fffffff;
-        unsigned long long who = __ballot(v == best);
+        const unsigned long long who = __ballot(v == best);
         if (who & (who - 1)) {
 #pragma unroll
             for (int s = 32; s; s >>= 1) list = min(list, __shfl_xor(list, s));
+            list = __builtin_amdgcn_readfirstlane(list);
         } else {
             list = __builtin_amdgcn_readlane(list, __ffsll(who) - 1);
         }
         int at = 0;
 #pragma unroll
+        for (int h = 0; h < HEADS; h++) at = list >> 6 == h ? __builtin_amdgcn_readlane(place[h], list & 63) : at;
+        const float after = at + 1 < (list + 1) * o.top ? s_list[at + 1] : NINF; // the list's next head
+#pragma unroll
         for (int h = 0; h < HEADS; h++) {
-            if (list == h * 64 + lane) {
-                at = next[h] - 1;
-                head[h] = next[h] < (list + 1) * o.top ? s_list[next[h]] : NINF;
-                next[h]++;
-            }
+            const bool taken = list == h * 64 + lane;
+            head[h] = taken ? after : head[h];
+            place[h] += taken ? 1 : 0;
         }
-        at = __builtin_amdgcn_readlane(at, list & 63);
-        if (lane == k) {
-            mine_v = best;
-            mine_i = s_index[at];
-        }
+        mine_v = lane == k ? best : mine_v;
+        mine_at = lane == k ? at : mine_at;
     }
     if (lane < o.top) {
-        o.top_logp[(size_t)row * o.top + lane] = mine_i < 0 ? NINF : mine_v - t.M - logS;
-        o.top_moves[(size_t)row * o.top + lane] = mine_i;
+        o.top_logp[(size_t)row * o.top + lane] = mine_at < 0 ? NINF : mine_v - t.M - logS;
+        o.top_moves[(size_t)row * o.top + lane] = mine_at < 0 ? -1 : s_index[mine_at];
     }
 }
 
@@ -828,16 +838,13 @@ template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_loss(Row
         }
     }
     const double v = value_part<T>(a, o, scale);
-    if (o.part) block_part(sum, v, o.part + 2 * (size_t)blockIdx.x);
+    if (o.part) block_part<WAVES>(sum, v, o.part + 2 * (size_t)blockIdx.x);
 }
 
 // ---------------------------------------------------------------- host side
 
 int launch_ok() { return hipGetLastError() == hipSuccess ? AZ_OK : AZ_ERR_HIP; }
 
-// Workgroups of a launch over `units` wavefronts' work: eight workgroups per CU fill it (8 x 4 wavefronts); more work
-// per wavefront comes by striding over the grid.
-constexpr int GRID_MAX = 256 * 8;
 int grid_of(long long units)
 {
     const long long b = (units + WAVES - 1) / WAVES;
@@ -1016,7 +1023,7 @@ int az_policy_loss(int n, int actions, const void *d_logits, int dtype, long lon
             hipLaunchKernelGGL((k_long_loss<T>), dim3(blocks), block, 0, st, a, c, (const Part *)w.part, o);
         });
     }
-    if (d_loss) hipLaunchKernelGGL(k_loss_join, dim3(1), block, 0, st, (const double *)d_work, blocks, 1. / n, d_loss, d_parts);
+    if (d_loss) hipLaunchKernelGGL(k_loss_join, dim3(1), dim3(64 * JOIN_WAVES), 0, st, (const double *)d_work, blocks, 1. / n, d_loss, d_parts);
     return launch_ok();
 }
 
