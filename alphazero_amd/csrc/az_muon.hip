@@ -28,8 +28,9 @@ namespace {
 
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr int EXP_X = 15, EXP_A = 14, EXP_Q = 10; // stored number = value * 2^EXP
-constexpr int MAX_BATCH = 64;                     // matrices per launch (their addresses travel as kernel arguments)
-constexpr int NORM_PARTS = 256;                   // partial sums of squares per matrix, at most
+constexpr int MAX_TABLE = 64;                     // matrices per launch when their addresses travel as kernel arguments
+constexpr int MAX_BATCH = 4096;                   // and at most
+constexpr int NORM_PARTS = 512;                   // partial sums of squares per matrix, at most
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f16v __attribute__((ext_vector_type(16)));
@@ -46,7 +47,18 @@ __device__ __forceinline__ void put(bf16_t *p, float v)
 }
 __device__ __forceinline__ void put(_Float16 *p, float v) { *p = (_Float16)v; }
 
-struct Ptrs { const void *in[MAX_BATCH]; void *out[MAX_BATCH]; };
+// the matrices' addresses: evenly spaced ones (a batch in one tensor) as first and distance, any number of them; others
+// as a table
+struct Ptrs {
+    const char *in0;
+    char *out0;
+    long long in_step, out_step;
+    int even;
+    const void *in_at[MAX_TABLE];
+    void *out_at[MAX_TABLE];
+    __device__ __forceinline__ const void *in(int i) const { return even ? in0 + i * in_step : in_at[i]; }
+    __device__ __forceinline__ void *out(int i) const { return even ? out0 + i * out_step : out_at[i]; }
+};
 
 // the matrices of a launch: G is rows x cols with row pitch ld (elements), X is G or its transpose, m x n with m <= n
 struct Shape {
@@ -58,7 +70,7 @@ struct Shape {
 // ---- sum of squares, in 64 bits (a float32 square leaves the range at 1e19 and 1e-23)
 template <class T> __global__ __launch_bounds__(256) void k_norm(Ptrs p, Shape s, int parts, double *sums)
 {
-    const T *g = (const T *)p.in[blockIdx.y];
+    const T *g = (const T *)p.in(blockIdx.y);
     double acc[4] = {0., 0., 0., 0.};
     // a wavefront takes pieces of 256 cells of a row
     const int pieces = (s.cols + 255) / 256;
@@ -98,7 +110,7 @@ template <class T> __global__ __launch_bounds__(256) void k_split(Ptrs p, Shape 
     __shared__ float t[64][65];
     __shared__ double s_scale;
     const int b = blockIdx.z;
-    const T *g = (const T *)p.in[b];
+    const T *g = (const T *)p.in(b);
     const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
     float v[16]; // all loads are in flight while the sum is taken
 #pragma unroll
@@ -145,7 +157,10 @@ struct Gemm {
     float alpha, beta, gamma;
     const char *E;      // packed, same shape as D; or NULL
     size_t sE, sD;
-    char *D;            // packed result, by columns: [N][M]; NULL: to p.out[] as G (columns: n, rows: m)
+    const char *A2, *B2; // a second product of the same shape in the same launch (no E), or NULL
+    char *D2;
+    int batch;
+    char *D;            // packed result, by columns: [N][M]; NULL: to p.out() as G (columns: n, rows: m)
     int pitchD;
 };
 
@@ -219,14 +234,24 @@ __device__ __forceinline__ void store_tile(float *t, const Gemm &a, const Ptrs &
 {
     const int row0 = ti * BM, col0 = tj * BN; // rows: m, columns: n
     if (!a.D) {
-        T *out = (T *)p.out[b];
-        for (int e = threadIdx.x; e < BM * BN; e += THREADS) {
-            if (s.tall) {
-                const int c = e / BM, r = e % BM;
-                if (row0 + r < s.m && col0 + c < s.n) put(out + (size_t)(col0 + c) * s.ld_out + row0 + r, t[tile_place<BM>(r, c)]);
-            } else { // 4 rows of 16 columns per wavefront: all banks
-                const int c = (e >> 6) % (BN / 16) * 16 + (e & 15), r = (e >> 6) / (BN / 16) * 4 + (e >> 4 & 3);
-                if (row0 + r < s.m && col0 + c < s.n) put(out + (size_t)(row0 + r) * s.ld_out + col0 + c, t[tile_place<BM>(r, c)]);
+        // 8 neighbours of a row of G per thread: along m where G is X', along n where it is X
+        T *out = (T *)p.out(b);
+        const bool wide = ((size_t)out | (size_t)s.ld_out * sizeof(T)) % 16 == 0; // whole 16-byte writes
+        for (int e = threadIdx.x; e < BM * BN / 8; e += THREADS) {
+            const int r = s.tall ? e % (BM / 8) * 8 : e / (BN / 8), c = s.tall ? e / (BM / 8) : e % (BN / 8) * 8;
+            __align__(16) T v[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) put(v + i, t[s.tall ? tile_place<BM>(r + (i & 4), c) + (i & 3) : tile_place<BM>(r, c + i)]);
+            const int left = s.tall ? s.m - row0 - r : s.n - col0 - c;
+            if (left <= 0 || (s.tall ? col0 + c >= s.n : row0 + r >= s.m)) continue;
+            T *at = s.tall ? out + (size_t)(col0 + c) * s.ld_out + row0 + r : out + (size_t)(row0 + r) * s.ld_out + col0 + c;
+            if (wide && left >= 8) {
+#pragma unroll
+                for (int i = 0; i < (int)sizeof(T) / 2; i++) ((uint4 *)at)[i] = ((const uint4 *)v)[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (i < left) at[i] = v[i];
             }
         }
         return;
@@ -284,6 +309,12 @@ __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs
         b = item / a.tiles;
         tile_at(item - b * a.tiles, a, ti, tj);
     }
+    if (a.D2 && b >= a.batch) {
+        a.A = a.A2;
+        a.B = a.B2;
+        a.D = a.D2;
+        b -= a.batch;
+    }
     const char *A = a.A + b * a.sA + (TURN ? (size_t)ti * BM * 4 : (size_t)ti * BM * a.pitchA);
     const char *B = a.B + b * a.sB + (TURN ? (size_t)tj * BN * 4 : (size_t)tj * BN * a.pitchB);
 
@@ -317,6 +348,9 @@ __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs
 #pragma unroll
         for (int l = 0; l < LOADS; l++) load_lds(src[l] + (size_t)k * (l * 4 < BM / 8 ? next_a : next_b), to + dst[l]);
     };
+    // A result of bfloat16 is rounded at 2^-9: its last product needs no small products (they are below 2^-11, and nothing
+    // multiplies that error any more).
+    constexpr bool LOW = !std::is_same<T, bf16_t>::value;
     // the small products have accumulators of their own: added to the large ones they would cost a rounding each
     // (three times the error of one step)
     f16v acc[FM][FN], low[FM][FN];
@@ -376,8 +410,10 @@ __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs
             for (int i = 0; i < FM; i++)
 #pragma unroll
                 for (int j = 0; j < FN; j++) {
-                    low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], low[i][j], 0, 0, 0);
-                    low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], low[i][j], 0, 0, 0);
+                    if (LOW) {
+                        low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], low[i][j], 0, 0, 0);
+                        low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], low[i][j], 0, 0, 0);
+                    }
                     acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
                 }
         }
@@ -392,7 +428,7 @@ __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs
             for (int e = 0; e < 16; e += 4) {
                 float v[4];
 #pragma unroll
-                for (int q = 0; q < 4; q++) v[q] = (acc[i][j][e + q] + low[i][j][e + q]) * a.alpha;
+                for (int q = 0; q < 4; q++) v[q] = (LOW ? acc[i][j][e + q] + low[i][j][e + q] : acc[i][j][e + q]) * a.alpha;
                 *(float4 *)(part + tile_place<BM>(wm + i * 32 + e * 2 + half * 4, wn + j * 32 + lr)) = make_float4(v[0], v[1], v[2], v[3]);
             }
     __syncthreads();
@@ -455,7 +491,7 @@ template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES
     h8 xh[NT][C], xl[NT][C];
     {
         float x[NT][C][8];
-        const T *g = (const T *)p.in[blockIdx.x];
+        const T *g = (const T *)p.in(blockIdx.x);
         const long long pm = s.tall ? 1 : s.ld_in, pn = s.tall ? s.ld_in : 1;
         double sum = 0.;
 #pragma unroll
@@ -651,7 +687,7 @@ template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES
             for (int c = 0; c < C; c++) split8(x[c], xh[t][c], xl[t][c]);
         }
     }
-    T *out = (T *)p.out[blockIdx.x];
+    T *out = (T *)p.out(blockIdx.x);
     const long long pm = s.tall ? 1 : s.ld_out, pn = s.tall ? s.ld_out : 1;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
@@ -711,6 +747,8 @@ Plan plan_of(const Shape &s, int batch)
 // launches D = alpha A B' + ... over `batch` matrices
 void gemm(Gemm a, int M, int N, bool turn, int batch, int dtype, const Ptrs &p, const Shape &s, hipStream_t st)
 {
+    a.batch = batch;
+    if (a.D2) batch *= 2;
     // 128 x 128 tiles halve the operand traffic of 64 x 64 ones, but a launch should have a workgroup for every CU
     const auto tiles = [&](int t) { return a.symmetric ? (long long)(M / t) * (M / t + 1) / 2 : (long long)(M / t) * (N / t); };
     const bool big = M % 128 == 0 && N % 128 == 0 && tiles(128) * batch >= 256;
@@ -772,8 +810,8 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
     char *XT = work + pl.sums, *YT = XT + batch * pl.x;
     char *mm[5];
     for (int i = 0; i < 5; i++) mm[i] = YT + batch * pl.x + i * batch * pl.mm;
-    // workgroups per matrix: eight pieces for each wavefront, or what fills the chip
-    long long parts_l = ((long long)s.rows * ((s.cols + 255) / 256) + 31) / 32;
+    // workgroups per matrix: two pieces for each wavefront, up to what their joining costs
+    const long long parts_l = ((long long)s.rows * ((s.cols + 255) / 256) + 7) / 8;
     const int parts = (int)(parts_l > NORM_PARTS ? NORM_PARTS : parts_l);
     const int rp = s.tall ? s.np : s.mp, cp = s.tall ? s.mp : s.np; // padded rows and columns of G
     by_type(dtype, [&](auto *d) {
@@ -785,7 +823,7 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
     const int pm = s.mp * 4;
     // a symmetric m x m product of two packed ones, 2^ex * 2^ey in the accumulator, stored with 2^eo
     const auto square = [&](const char *x, int ex, const char *y, int ey, char *out, int eo, float f = 1.f, const char *E = nullptr,
-                            float beta = 0.f, float gamma = 0.f) {
+                            float beta = 0.f, float gamma = 0.f, const char *x2 = nullptr, const char *y2 = nullptr, char *out2 = nullptr) {
         Gemm g = {};
         g.A = x; g.B = y;
         g.sA = g.sB = g.sE = g.sD = pl.mm;
@@ -795,12 +833,14 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
         g.alpha = f * two(eo - ex - ey);
         g.E = E; g.beta = beta; g.gamma = gamma;
         g.D = out;
+        g.A2 = x2; g.B2 = y2; g.D2 = out2;
         gemm(g, s.mp, s.mp, false, batch, dtype, p, s, st);
     };
-    // Steps per group.  Results of 16 bits (half a step: 2^-9, 2^-12) have room for three.  For float32 groups of two
-    // keep the error where single steps have it and pay where X is much wider than high: at n = 4 m they leave 47
-    // of 65 m^3 products, at n = 2 m 29 of 35.
-    const int group = dtype != AZ_F32 ? 3 : s.n >= 4 * s.m ? 2 : 1;
+    // Steps per group.  Results of 16 bits (half a step: 2^-9, 2^-12) have room for three, which pay as soon as X is wider
+    // than high: at n = 1.5 m 23 m^3 products are left of 27.5 (five steps), at n = 4 m 38 of 65.  For float32 groups of
+    // two keep the error where single steps have it and pay where X is much wider than high: at n = 4 m they leave
+    // 47 of 65, at n = 2 m 29 of 35.
+    const int group = dtype != AZ_F32 ? (2 * s.n >= 3 * s.m ? 3 : 1) : s.n >= 4 * s.m ? 2 : 1;
     for (int left = steps; left > 0;) {
         // (the odd ones first: the longer groups start from the better conditioned matrix)
         const int k = left > group ? (left % group ? left % group : group) : left;
@@ -821,21 +861,25 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
         const auto poly = [&](char *out) { // a I + b A + c A^2
             square(A, EXP_A, A, EXP_A, out, EXP_Q, NS_C, A, NS_B * two(EXP_Q - EXP_A), NS_A * two(EXP_Q));
         };
+        // W, V: Q of the group's latest steps; the product of all of them ends in `total`
         poly(W);
-        for (int i = 1; i < k; i++) {
-            // W = the last step's Q; A <- (A W) W, V = the next step's Q, Q = the product of all so far
+        const char *total = W;
+        if (k > 1) {
             square(A, EXP_A, W, EXP_Q, T, EXP_A);
             square(T, EXP_A, W, EXP_Q, A, EXP_A);
             poly(V);
-            square(V, EXP_Q, i == 1 ? W : Q, EXP_Q, T, EXP_Q);
-            char *old = Q;
-            Q = T;
-            T = old;
-            char *w = W;
-            W = V;
-            V = w;
+            if (k == 2) {
+                square(V, EXP_Q, W, EXP_Q, Q, EXP_Q);
+                total = Q;
+            } else { // Q = V W and T = A V do not wait for each other
+                static_assert(EXP_Q - 2 * EXP_Q == EXP_A - EXP_A - EXP_Q, "one factor for both");
+                square(V, EXP_Q, W, EXP_Q, Q, EXP_Q, 1.f, nullptr, 0.f, 0.f, A, V, T);
+                square(T, EXP_A, V, EXP_Q, A, EXP_A);
+                poly(W);
+                square(W, EXP_Q, Q, EXP_Q, T, EXP_Q);
+                total = T;
+            }
         }
-        const char *total = k == 1 ? W : Q;
         left -= k;
         Gemm g = {}; // X <- Q X, by columns
         g.A = total; g.B = XT;
@@ -856,16 +900,23 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
     return launch_ok();
 }
 
-// Matrices per batch: as many as the kernel arguments hold, but no more than a workspace of 1 GiB needs (matrices that
-// large fill the chip one by one).
+// Matrices per launch: a workspace of 1 GiB at most (matrices that large fill the chip one by one)
 int batch_of(const Shape &s, int count)
 {
-    if (is_small(s)) return count < MAX_BATCH ? count : MAX_BATCH;
-    const size_t one = plan_of(s, 1).total;
-    long long most = (long long)(((size_t)1 << 30) / one);
-    if (most < 1) most = 1;
-    if (most > MAX_BATCH) most = MAX_BATCH;
+    long long most = MAX_BATCH;
+    if (!is_small(s)) {
+        const long long fit = (long long)(((size_t)1 << 30) / plan_of(s, 1).total);
+        most = fit < 1 ? 1 : fit < most ? fit : most;
+    }
     return (int)(count < most ? count : most);
+}
+
+// whether n addresses are evenly spaced
+bool spaced(const void *const *p, int n)
+{
+    for (int i = 2; i < n; i++)
+        if ((const char *)p[i] - (const char *)p[i - 1] != (const char *)p[1] - (const char *)p[0]) return false;
+    return true;
 }
 
 } // namespace
@@ -894,15 +945,25 @@ int az_muon_orthogonalise(int count, int rows, int cols, const void *const *d_in
     const bool small = is_small(s);
     if (!small && !d_work) return AZ_ERR_ARG;
     const int batch = batch_of(s, count);
-    for (int at = 0; at < count; at += batch) {
-        const int n = count - at < batch ? count - at : batch;
+    for (int at = 0; at < count;) {
+        int n = count - at < batch ? count - at : batch;
         Ptrs p = {};
-        for (int i = 0; i < n; i++) {
-            p.in[i] = d_in[at + i];
-            p.out[i] = d_out[at + i];
+        p.even = spaced(d_in + at, n) && spaced(d_out + at, n);
+        if (!p.even && n > MAX_TABLE) n = MAX_TABLE;
+        if (p.even) {
+            p.in0 = (const char *)d_in[at];
+            p.out0 = (char *)d_out[at];
+            p.in_step = n > 1 ? (const char *)d_in[at + 1] - p.in0 : 0;
+            p.out_step = n > 1 ? (char *)d_out[at + 1] - p.out0 : 0;
+        } else {
+            for (int i = 0; i < n; i++) {
+                p.in_at[i] = d_in[at + i];
+                p.out_at[i] = d_out[at + i];
+            }
         }
         const int rc = small ? run_small(n, s, dtype, steps, p, (hipStream_t)stream) : run_batch(n, s, dtype, steps, p, (char *)d_work, (hipStream_t)stream);
         if (rc != AZ_OK) return rc;
+        at += n;
     }
     return AZ_OK;
 }
