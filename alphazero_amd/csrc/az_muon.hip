@@ -493,20 +493,46 @@ template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES
         float x[NT][C][8];
         const T *g = (const T *)p.in(blockIdx.x);
         const long long pm = s.tall ? 1 : s.ld_in, pn = s.tall ? s.ld_in : 1;
+        // (no branch around a load: all of them are in flight together; a row number that is the same in all lanes but for
+        // their half is a scalar offset)
+        const auto load = [&](auto full) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const int n = (t * SMALL_WAVES + wave) * 32 + lr;
+                const T *col = g + min(n, s.n - 1) * pn + (decltype(full)::value ? 4 * half * pm : 0);
+#pragma unroll
+                for (int c = 0; c < C; c++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int m = c * 16 + 8 * (e >> 2) + (e & 3);
+                        if (decltype(full)::value) {
+                            const float v = as_float(col[m * pm]);
+                            x[t][c][e] = n < s.n ? v : 0.f;
+                        } else {
+                            const float v = as_float(col[min(m + 4 * half, s.m - 1) * pm]);
+                            x[t][c][e] = m + 4 * half < s.m && n < s.n ? v : 0.f;
+                        }
+                    }
+            }
+        };
+        if (s.m == M && s.tall) { // a lane's rows lie side by side in fours
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const int n = (t * SMALL_WAVES + wave) * 32 + lr;
+                const T *col = g + min(n, s.n - 1) * pn + 4 * half;
+#pragma unroll
+                for (int c = 0; c < C; c++)
+#pragma unroll
+                    for (int e = 0; e < 8; e += 4) {
+                        T four[4];
+                        __builtin_memcpy(four, col + c * 16 + 2 * e, sizeof(four));
+#pragma unroll
+                        for (int i = 0; i < 4; i++) x[t][c][e + i] = n < s.n ? as_float(four[i]) : 0.f;
+                    }
+            }
+        } else if (s.m == M) load(std::true_type());
+        else load(std::false_type());
         double sum = 0.;
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-            const int n = (t * SMALL_WAVES + wave) * 32 + lr;
-            const T *col = g + min(n, s.n - 1) * pn;
-#pragma unroll
-            for (int c = 0; c < C; c++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int m = c * 16 + 8 * (e >> 2) + 4 * half + (e & 3);
-                    const float v = as_float(col[min(m, s.m - 1) * pm]); // (no branch: all loads are in flight together)
-                    x[t][c][e] = m < s.m && n < s.n ? v : 0.f;
-                }
-        }
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -521,13 +547,16 @@ template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES
 #pragma unroll
         for (int w = 0; w < SMALL_WAVES; w++) sum += ((double *)lds)[w];
         __syncthreads();
-        const double scale = sum == 0. ? 0. : ldexp(1. / sqrt(sum), EXP_X);
+        // 1 / |X| = f 2^k with f in [1/2, 1]: a float32 product, rounded once, and a power of two
+        int k;
+        const float f = sum == 0. ? 0.f : (float)frexp(1. / sqrt(sum), &k);
+        k = sum == 0. ? 0 : k + EXP_X;
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int c = 0; c < C; c++) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) x[t][c][e] = (float)((double)x[t][c][e] * scale);
+                for (int e = 0; e < 8; e++) x[t][c][e] = ldexpf(x[t][c][e] * f, k);
                 split8(x[t][c], xh[t][c], xl[t][c]);
             }
     }
@@ -689,18 +718,40 @@ template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES
     }
     T *out = (T *)p.out(blockIdx.x);
     const long long pm = s.tall ? 1 : s.ld_out, pn = s.tall ? s.ld_out : 1;
+    const auto store = [&](auto full) {
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
-        const int n = (t * SMALL_WAVES + wave) * 32 + lr;
+        for (int t = 0; t < NT; t++) {
+            const int n = (t * SMALL_WAVES + wave) * 32 + lr;
+            if (n >= s.n) continue;
+            T *col = out + n * pn + 4 * half * pm;
 #pragma unroll
-        for (int c = 0; c < C; c++)
+            for (int c = 0; c < C; c++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int m = c * 16 + 8 * (e >> 2) + 4 * half + (e & 3);
-                const float v = ((float)xh[t][c][e] + (float)xl[t][c][e]) * 0x1p-15f; // 2^-EXP_X
-                if (m < s.m && n < s.n) put(out + n * pn + m * pm, v);
-            }
-    }
+                for (int e = 0; e < 8; e++) {
+                    const int m = c * 16 + 8 * (e >> 2) + (e & 3);
+                    const float v = ((float)xh[t][c][e] + (float)xl[t][c][e]) * 0x1p-15f; // 2^-EXP_X
+                    if (decltype(full)::value || m + 4 * half < s.m) put(col + m * pm, v);
+                }
+        }
+    };
+    if (s.m == M && s.tall) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const int n = (t * SMALL_WAVES + wave) * 32 + lr;
+            if (n >= s.n) continue;
+            T *col = out + n * pn + 4 * half;
+#pragma unroll
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int e = 0; e < 8; e += 4) {
+                    T four[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) put(four + i, ((float)xh[t][c][e + i] + (float)xl[t][c][e + i]) * 0x1p-15f);
+                    __builtin_memcpy(col + c * 16 + 2 * e, four, sizeof(four));
+                }
+        }
+    } else if (s.m == M) store(std::true_type());
+    else store(std::false_type());
 }
 static_assert(EXP_X == 15 && EXP_A == 14 && EXP_Q == 10, "the powers of two written out in k_small");
 
