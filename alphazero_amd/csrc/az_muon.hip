@@ -9,7 +9,7 @@
 // and every m x m product computes its upper tiles only: 3 m^2 n + (4k - 3) m^3 products a group.  What limits k is that a
 // Gram matrix carries an error of 2^-24 |A| into directions whose singular value is near 0, where a step multiplies it
 // by a^2 = 11.9.  Measured error of five steps against 64 bits, next to float32 products (16 x 144, 256 x 256, 256 x
-// 2304):  k = 1  0.9, 0.4, 0.7 times;  k = 2  0.8, 1.2, 1.0;  k = 3  3.2, 11, 0.7.
+// 2304):  k = 1  0.9, 0.4, 0.7 times;  k = 2  0.8, 1.2, 1.0 (2.5 on an update of low rank);  k = 3  3.2, 11, 0.7.
 //
 // Arithmetic: the matrix cores have no fast float32 product, so a number is held as the sum of two float16 numbers
 // (hi + lo, 22 bits) times a power of two, and a product is hi hi + hi lo + lo hi in float32 accumulators (the missing
@@ -887,11 +887,10 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
         g.A2 = x2; g.B2 = y2; g.D2 = out2;
         gemm(g, s.mp, s.mp, false, batch, dtype, p, s, st);
     };
-    // Steps per group.  Results of 16 bits (half a step: 2^-9, 2^-12) have room for three, which pay as soon as X is wider
-    // than high: at n = 1.5 m 23 m^3 products are left of 27.5 (five steps), at n = 4 m 38 of 65.  For float32 groups of
-    // two keep the error where single steps have it and pay where X is much wider than high: at n = 4 m they leave
-    // 47 of 65, at n = 2 m 29 of 35.
-    const int group = dtype != AZ_F32 ? (2 * s.n >= 3 * s.m ? 3 : 1) : s.n >= 4 * s.m ? 2 : 1;
+    // Steps per group.  float32 results take every step on X (the error stays at or below that of float32 products).
+    // Results of 16 bits (half a step: 2^-9, 2^-12) have room for three, which pay as soon as X is wider than high: of five
+    // steps' 27.5 m^3 products at n = 1.5 m 23 are left, of 65 at n = 4 m 38.
+    const int group = dtype != AZ_F32 && 2 * s.n >= 3 * s.m ? 3 : 1;
     for (int left = steps; left > 0;) {
         // (the odd ones first: the longer groups start from the better conditioned matrix)
         const int k = left > group ? (left % group ? left % group : group) : left;

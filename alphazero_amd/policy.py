@@ -263,6 +263,8 @@ def loss(logits, value, pi, r, *, board=None, legal=None, parts=False):
     if n == 0:
         zero = logits.sum(dtype=torch.float32) + value.sum(dtype=torch.float32)
         return (zero, zero.detach(), zero.detach()) if parts else zero
+    if not torch.is_grad_enabled():
+        logits, value = logits.detach(), value.detach()  # no gradients are computed that nobody can ask for
     total, two = _LossFunction.apply(logits, value.contiguous(), pi.contiguous(), r.contiguous(), board, legal, bool(parts),
                                      rows, device)
     return (total, two[0], two[1]) if parts else total

@@ -124,6 +124,57 @@ def test_strides_lists_and_empty():
     assert not muon.orthogonalise(x).requires_grad
 
 
+def test_many_separate_tensors_and_odd_alignment():
+    # more tensors than one launch's table of addresses holds, none of them evenly spaced; rows that start at any element
+    from alphazero_amd import muon
+
+    store = _updates((1, 400000), 12).cuda().flatten()
+    at, many = 0, []
+    for i in range(70):
+        many.append(store[at:at + 64 * 70].view(64, 70))
+        at += 64 * 70 + i % 5 + 1
+    got = muon.orthogonalise(many)
+    for i in (0, 1, 33, 63, 64, 69):
+        _check(got[i], many[i])
+        assert torch.equal(got[i], muon.orthogonalise(many[i]))
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        flat = store[:200003].to(dtype)
+        for rows, cols, off in ((64, 129, 1), (129, 64, 3), (32, 65, 1), (130, 201, 1), (201, 130, 3)):
+            g = flat[off:off + rows * (cols + 2)].view(rows, cols + 2)[:, 1:cols + 1]
+            _check(muon.orthogonalise(g), g)
+
+
+def test_in_place_through_the_c_entry():
+    import ctypes as C
+
+    from alphazero_amd import engine as E
+    from alphazero_amd import muon
+
+    L = E.load_library()
+    for shape in ((3, 20, 50), (2, 100, 130)):
+        g = _updates(shape, 14).cuda()
+        want = muon.orthogonalise(g)
+        work = torch.empty(max(1, L.az_muon_work(*shape)), dtype=torch.uint8, device="cuda")
+        at = (C.c_void_p * shape[0])(*[t.data_ptr() for t in g])
+        rc = L.az_muon_orthogonalise(*shape, at, shape[2], at, shape[2], 0, 5, work.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and torch.equal(g, want)
+
+
+def test_two_streams_at_once():
+    from alphazero_amd import muon
+
+    gs = [_updates((2, 130, 300), 15).cuda(), _updates((9, 40, 300), 16).cuda()]
+    want = [muon.orthogonalise(g) for g in gs]
+    streams = [torch.cuda.Stream() for _ in gs]
+    torch.cuda.synchronize()
+    got = []
+    for k in range(6):
+        with torch.cuda.stream(streams[k % 2]):
+            got.append(muon.orthogonalise(gs[k % 2]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, want[k % 2]) for k, t in enumerate(got))
+
+
 def test_streams_and_graph_replay():
     from alphazero_amd import muon
 
@@ -168,6 +219,9 @@ def test_optimiser_step_by_step():
             want[i] = want[i] * (1 - 0.1 * 0.01) - 0.1 * max(1.0, g.shape[0] / g[0].numel()) ** 0.5 * u
     for p, t in zip(w, want):
         assert (p.detach().cpu().double() - t).norm() < 1e-5 * t.norm()
+    empty = torch.nn.Parameter(torch.zeros(3, 0, device="cuda"))
+    empty.grad = torch.zeros_like(empty)
+    muon.Muon([empty]).step()
     with pytest.raises(ValueError, match="two or more"):
         muon.Muon([torch.nn.Parameter(torch.zeros(4))])
 
