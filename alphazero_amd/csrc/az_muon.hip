@@ -455,7 +455,8 @@ __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs
 // instruction leaves a result), as hi and lo halves.  In that order a tile is at once the operand of the next Q X: only
 // Q's columns have to be stored in the same order.  For the Gram matrix the tile is turned through LDS (rows to lanes)
 // by transposing reads, every wavefront adds up its own columns and the eight partial sums meet in LDS in a fixed order.  Launches bound the general path here
-// (17 of them, 5 us each); this one is bound by the latency of 4 barriers a step and by one CU's matrix cores.
+// (17 of them, 5 us each); this one is bound by the latency of 3 barriers a step (2 up to 32 rows) and
+// by one CU's matrix cores and its share of the memory (11 of 40 us at 64 x 576 go into reading and writing).
 constexpr int SMALL_WAVES = 8;
 
 // 16-byte piece of a row of M * 4 bytes: rows spread over the banks
@@ -472,8 +473,6 @@ __device__ __forceinline__ void split8(const float *v, h8 &hi, h8 &lo)
     }
 }
 
-typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-
 __device__ __forceinline__ int row_of(int r) { return (r & ~12) | (r & 4) << 1 | (r & 8) >> 1; }
 
 template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES, 2) void k_small(Ptrs p, Shape s, int steps)
@@ -481,10 +480,10 @@ template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES
     constexpr int M = 32 * MT, LD = M + 8, C = 2 * MT; // C: blocks of 16 rows
     constexpr int TURN = 32 * LD * 2;                  // one half (hi or lo) of a tile, [column][row], rows 16 bytes apart
     constexpr int AREA = M * M * 4 > 2 * TURN ? M * M * 4 : 2 * TURN;
-    __shared__ __align__(16) char lds[SMALL_WAVES * AREA + M * M * 4];
+    __shared__ __align__(16) char lds[SMALL_WAVES * AREA + MT * M * M * 4]; // (MT == 2: all 160 KB of a CU)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lr = lane & 31, half = lane >> 5;
-    char *area = lds + wave * AREA, *sA = lds, *sQ = lds + SMALL_WAVES * AREA;
+    char *area = lds + wave * AREA, *sA = lds + SMALL_WAVES * AREA, *sQ = sA + M * M * 4;
     const int tiles = (s.n + 31) / 32;
 
     // X and |X|.  A lane's registers hold, of each block of 16 rows, rows 4 half + {0..3, 8..11}: hi and lo, 8 each
@@ -589,24 +588,16 @@ template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES
                     lo[i][c] = turned(area + TURN + at, area + TURN + at + 4 * LD * 2);
                 }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            // (instructions on the same accumulator wait for each other: the tiles in turn)
 #pragma unroll
-            for (int i = 0, q = 0; i < MT; i++)
+            for (int c = 0; c < 2; c++)
 #pragma unroll
-                for (int j = i; j < MT; j++, q++) {
-                    // the small products first, then the large ones on top, then one addition per 32 columns
-                    f16v acc;
+                for (int k = 0; k < 3; k++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) acc[e] = 0.f;
+                    for (int i = 0, q = 0; i < MT; i++)
 #pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo[i][c], hi[j][c], acc, 0, 0, 0);
-                        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi[i][c], lo[j][c], acc, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int c = 0; c < 2; c++) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi[i][c], hi[j][c], acc, 0, 0, 0);
-#pragma unroll
-                    for (int e = 0; e < 16; e++) gram[q][e] += acc[e];
-                }
+                        for (int j = i; j < MT; j++, q++)
+                            gram[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k == 0 ? lo[i][c] : hi[i][c], k == 1 ? lo[j][c] : hi[j][c], gram[q], 0, 0, 0);
         }
         // partial sums to the wavefront's own area, row c holding column c (the matrix is symmetric)
 #pragma unroll
@@ -642,18 +633,18 @@ template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES
             }
 #pragma unroll
             for (int k = 0; k < 8; k++) v[k] = ldexpf(v[k], EXP_A - 2 * EXP_X);
-        }
-        __syncthreads();
-        if (mine) {
             h8 hi, lo;
             split8(v, hi, lo);
             *(h8 *)(sA + r * M * 4 + bank<M>(r, slot(c16, h)) * 16) = hi;
             *(h8 *)(sA + r * M * 4 + bank<M>(r, slot(c16, h) + 1) * 16) = lo;
         }
         __syncthreads();
-        // Q = a I + b A + c A^2, one 32 x 32 tile per wavefront
-        if (wave < MT * MT) {
-            const int i = wave / MT, j = wave % MT, ra = i * 32 + lr, rb = j * 32 + lr;
+        // Q = a I + b A + c A^2: one 32 x 32 tile per wavefront, or the only tile in every one.  A lane's results are four
+        // rows side by side of its column, so (Q is symmetric) the 8 of a block are an operand's share of row `rb`, and
+        // so are the elements of A that go with them.
+        h8 qh1[2], ql1[2];
+        if (MT == 1 ? wave < tiles : wave < MT * MT) {
+            const int i = MT == 1 ? 0 : wave / MT, j = MT == 1 ? 0 : wave % MT, ra = i * 32 + lr, rb = j * 32 + lr;
             f16v acc;
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[e] = 0.f;
@@ -670,48 +661,57 @@ template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES
 #pragma unroll
             for (int c = 0; c < C; c++) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[c], bh[c], acc, 0, 0, 0);
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const int row = i * 32 + 2 * e + 4 * half; // rows row..row+3 of column rb, stored as row rb
-                const int at = rb * M * 4 + (e >> 2 & 1) * 8, pc = slot(row >> 4, half);
-                const h4 hi = *(const h4 *)(sA + at + bank<M>(rb, pc) * 16), lo = *(const h4 *)(sA + at + bank<M>(rb, pc + 1) * 16);
-                h4 qh, ql;
+            for (int c = 0; c < 2; c++) {
+                const char *at = sA + rb * M * 4;
+                const h8 hi = *(const h8 *)(at + bank<M>(rb, slot(2 * i + c, half)) * 16), lo = *(const h8 *)(at + bank<M>(rb, slot(2 * i + c, half) + 1) * 16);
+                float f[8];
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    float f = acc[e + k] * (NS_C * 0x1p-18f); // 2^(EXP_Q - 2 EXP_A)
-                    f = fmaf((float)hi[k] + (float)lo[k], NS_B * 0x1p-4f, f);
-                    if (row + k == rb) f += NS_A * 0x1p10f;
-                    qh[k] = (_Float16)f;
-                    ql[k] = (_Float16)(f - (float)qh[k]);
+                for (int k = 0; k < 8; k++) {
+                    f[k] = fmaf((float)hi[k] + (float)lo[k], NS_B * 0x1p-4f, acc[8 * c + k] * (NS_C * 0x1p-18f)); // 2^(EXP_Q - EXP_A), 2^(EXP_Q - 2 EXP_A)
+                    if (i * 32 + 16 * c + 8 * (k >> 2) + 4 * half + (k & 3) == rb) f[k] += NS_A * 0x1p10f;
                 }
-                *(h4 *)(sQ + at + bank<M>(rb, pc) * 16) = qh;
-                *(h4 *)(sQ + at + bank<M>(rb, pc + 1) * 16) = ql;
+                split8(f, qh1[c], ql1[c]);
+                if (MT > 1) {
+                    *(h8 *)(sQ + rb * M * 4 + bank<M>(rb, slot(2 * i + c, half)) * 16) = qh1[c];
+                    *(h8 *)(sQ + rb * M * 4 + bank<M>(rb, slot(2 * i + c, half) + 1) * 16) = ql1[c];
+                }
             }
         }
-        __syncthreads();
+        if (MT > 1) __syncthreads();
         // X <- Q X
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             if (t * SMALL_WAVES + wave >= tiles) continue;
             float x[C][8];
+            f16v acc[MT];
 #pragma unroll
-            for (int i = 0; i < MT; i++) {
-                const int rq = i * 32 + lr;
-                f16v acc;
+            for (int i = 0; i < MT; i++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) acc[e] = 0.f;
-                h8 qh[C];
+                for (int e = 0; e < 16; e++) acc[i][e] = 0.f;
+            // the small products first, then the large ones on top; the row blocks in turn
+            h8 qh[MT][C];
 #pragma unroll
-                for (int c = 0; c < C; c++) {
-                    qh[c] = *(const h8 *)(sQ + rq * M * 4 + bank<M>(rq, slot(c, half)) * 16);
-                    const h8 ql = *(const h8 *)(sQ + rq * M * 4 + bank<M>(rq, slot(c, half) + 1) * 16);
-                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql, xh[t][c], acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[c], xl[t][c], acc, 0, 0, 0);
+            for (int c = 0; c < C; c++) {
+                h8 ql[MT];
+#pragma unroll
+                for (int i = 0; i < MT; i++) {
+                    const int rq = i * 32 + lr;
+                    qh[i][c] = MT == 1 ? qh1[c] : *(const h8 *)(sQ + rq * M * 4 + bank<M>(rq, slot(c, half)) * 16);
+                    ql[i] = MT == 1 ? ql1[c] : *(const h8 *)(sQ + rq * M * 4 + bank<M>(rq, slot(c, half) + 1) * 16);
                 }
 #pragma unroll
-                for (int c = 0; c < C; c++) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[c], xh[t][c], acc, 0, 0, 0);
+                for (int i = 0; i < MT; i++) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[i], xh[t][c], acc[i], 0, 0, 0);
 #pragma unroll
-                for (int e = 0; e < 16; e++) x[2 * i + (e >> 3)][e & 7] = acc[e] * 0x1p-10f; // 2^-EXP_Q
+                for (int i = 0; i < MT; i++) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[i][c], xl[t][c], acc[i], 0, 0, 0);
             }
+#pragma unroll
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int i = 0; i < MT; i++) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[i][c], xh[t][c], acc[i], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) x[2 * i + (e >> 3)][e & 7] = acc[i][e] * 0x1p-10f; // 2^-EXP_Q
 #pragma unroll
             for (int c = 0; c < C; c++) split8(x[c], xh[t][c], xl[t][c]);
         }

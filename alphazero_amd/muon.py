@@ -34,12 +34,13 @@ def _on_gpu(tensors):
 
 
 def _run(inputs, outputs, rows, cols, ld, dtype, device, steps):
-    """inputs, outputs: device addresses of matrices of one shape, rows `ld` (outputs: cols) elements apart."""
+    """inputs, outputs: device addresses of matrices of one shape on GPU `device` (an index), rows `ld` (outputs: cols)
+    elements apart."""
     count = len(inputs)
     addresses = C.c_void_p * count
     size = _work(count, rows, cols)
-    work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    _call("az_muon_orthogonalise", device.index, count, rows, cols, addresses(*inputs), ld, addresses(*outputs), cols,
+    work = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", device)) if size else None
+    _call("az_muon_orthogonalise", device, count, rows, cols, addresses(*inputs), ld, addresses(*outputs), cols,
           TYPES[dtype], steps, _ptr(work))
 
 
@@ -51,7 +52,6 @@ def _rows_apart(x):
     return x, x.stride(-2) if rows > 1 else cols
 
 
-@torch.no_grad()
 def orthogonalise(updates, steps=5):
     """Moves the singular values of each update towards 1 and keeps its singular vectors: X = G / |G|, then `steps` times
     X <- a X + (b A + c A^2) X with A = X X' and (a, b, c) = (3.4445, -4.7750, 2.0315).
@@ -68,12 +68,12 @@ def orthogonalise(updates, steps=5):
         _on_gpu([updates])
         out = updates.new_empty(updates.shape)
         if out.numel():
-            x, ld = _rows_apart(updates)
+            x, ld = _rows_apart(updates.detach())
             size = x.element_size()
             count = x.shape[0] if x.dim() == 3 else 1
             step = x.stride(0) * size if x.dim() == 3 else 0
             a, b, c = x.data_ptr(), out.data_ptr(), rows * cols * size
-            _run([a + i * step for i in range(count)], [b + i * c for i in range(count)], rows, cols, ld, x.dtype, x.device, steps)
+            _run([a + i * step for i in range(count)], range(b, b + count * c, c), rows, cols, ld, x.dtype, x.get_device(), steps)
         return out
     updates = list(updates)
     groups = {}
@@ -86,8 +86,8 @@ def orthogonalise(updates, steps=5):
     for i, t in enumerate(updates):
         outs.append(torch.empty(t.shape, dtype=t.dtype, device=t.device))
         if t.numel():
-            x, ld = _rows_apart(t.flatten(1))
-            groups.setdefault((x.shape[0], x.shape[1], ld, x.dtype, x.device), []).append((x, outs[i]))
+            x, ld = _rows_apart(t.detach().flatten(1))
+            groups.setdefault((x.shape[0], x.shape[1], ld, x.dtype, x.get_device()), []).append((x, outs[i]))
     for (rows, cols, ld, dtype, device), members in groups.items():
         _run([x.data_ptr() for x, _ in members], [o.data_ptr() for _, o in members], rows, cols, ld, dtype, device, steps)
     return outs
