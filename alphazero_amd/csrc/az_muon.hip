@@ -30,6 +30,7 @@ constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr int EXP_X = 15, EXP_A = 14, EXP_Q = 10; // stored number = value * 2^EXP
 constexpr int MAX_TABLE = 64;                     // matrices per launch when their addresses travel as kernel arguments
 constexpr int MAX_BATCH = 4096;                   // and at most
+constexpr int BIG_TILES = 256;                    // 128 x 128 tiles from this number of them on: one for every CU
 constexpr int NORM_PARTS = 512;                   // partial sums of squares per matrix, at most
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -105,7 +106,8 @@ __device__ __forceinline__ void pack8(char *p, const float (&v)[8])
     *(h8 *)(p + 16) = lo;
 }
 // X' = the packed transpose of G / |G| (G itself, row by row, when it is tall), [np][mp]; one 64 x 64 tile of G per workgroup
-template <class T> __global__ __launch_bounds__(256) void k_split(Ptrs p, Shape s, int parts, const double *sums, char *XT)
+// (X: also X itself, [mp][np], or NULL)
+template <class T> __global__ __launch_bounds__(256) void k_split(Ptrs p, Shape s, int parts, const double *sums, char *XT, char *X)
 {
     __shared__ float t[64][65];
     __shared__ double s_scale;
@@ -143,6 +145,12 @@ template <class T> __global__ __launch_bounds__(256) void k_split(Ptrs p, Shape 
 #pragma unroll
         for (int i = 0; i < 8; i++) w[i] = t[n][m + i];
         if (n0 + n < s.np && m0 + m < s.mp) pack8(out + ((size_t)(n0 + n) * s.mp + m0 + m) * 4, w);
+        if (X) {
+            const int r = e >> 3, c = (e & 7) * 8; // row of X, columns
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[i] = t[c + i][r];
+            if (m0 + r < s.mp && n0 + c < s.np) pack8(X + b * ((size_t)s.mp * s.np * 4) + ((size_t)(m0 + r) * s.np + n0 + c) * 4, w);
+        }
     }
 }
 
@@ -160,6 +168,8 @@ struct Gemm {
     const char *A2, *B2; // a second product of the same shape in the same launch (no E), or NULL
     char *D2;
     int batch;
+    char *M;            // the packed result by rows too, [M][N], or NULL
+    int pitchM;
     char *D;            // packed result, by columns: [N][M]; NULL: to p.out() as G (columns: n, rows: m)
     int pitchD;
 };
@@ -273,14 +283,16 @@ __device__ __forceinline__ void store_tile(float *t, const Gemm &a, const Ptrs &
         }
         pack8(D + at, v);
     }
-    if (!a.symmetric || ti == tj) return;
+    if (a.symmetric ? ti == tj : a.M == nullptr) return;
+    char *M = a.symmetric ? D : a.M + b * a.sD;
+    const int pitch = a.symmetric ? a.pitchD : a.pitchM;
     __syncthreads();
     for (int e = threadIdx.x; e < BM * BN / 8; e += THREADS) {
         const int r = e / (BN / 8), c = e % (BN / 8) * 8;
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = t[tile_place<BM>(r, c + i)];
-        pack8(D + (size_t)(row0 + r) * a.pitchD + (size_t)(col0 + c) * 4, v);
+        pack8(M + (size_t)(row0 + r) * pitch + (size_t)(col0 + c) * 4, v);
     }
 }
 
@@ -791,7 +803,7 @@ Plan plan_of(const Shape &s, int batch)
     p.x = (size_t)s.mp * s.np * 4;
     p.mm = (size_t)s.mp * s.mp * 4;
     p.sums = (size_t)batch * NORM_PARTS * sizeof(double);
-    p.total = p.sums + batch * (2 * p.x + 5 * p.mm);
+    p.total = p.sums + batch * (3 * p.x + 5 * p.mm);
     return p;
 }
 
@@ -802,7 +814,7 @@ void gemm(Gemm a, int M, int N, bool turn, int batch, int dtype, const Ptrs &p, 
     if (a.D2) batch *= 2;
     // 128 x 128 tiles halve the operand traffic of 64 x 64 ones, but a launch should have a workgroup for every CU
     const auto tiles = [&](int t) { return a.symmetric ? (long long)(M / t) * (M / t + 1) / 2 : (long long)(M / t) * (N / t); };
-    const bool big = M % 128 == 0 && N % 128 == 0 && tiles(128) * batch >= 256;
+    const bool big = M % 128 == 0 && N % 128 == 0 && tiles(128) * batch >= BIG_TILES;
     const int t = big ? 128 : 64;
     const long long groups = tiles(t) * batch;
     a.tiles = (int)tiles(t);
@@ -858,9 +870,14 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
 {
     const Plan pl = plan_of(s, batch);
     double *sums = (double *)work;
-    char *XT = work + pl.sums, *YT = XT + batch * pl.x;
+    char *XT = work + pl.sums, *YT = XT + batch * pl.x, *X = YT + batch * pl.x;
     char *mm[5];
-    for (int i = 0; i < 5; i++) mm[i] = YT + batch * pl.x + i * batch * pl.mm;
+    for (int i = 0; i < 5; i++) mm[i] = X + batch * pl.x + i * batch * pl.mm;
+    // Transposing LDS reads are half as fast as plain ones.  That does not matter where loads are waited for, but a Gram
+    // matrix of large tiles is bound by LDS with them: there X is kept by rows as well (4096 x 4096 4.89 -> 4.55 ms,
+    // 2 x 2048 x 4096 2.34 -> 2.23 ms, 8 x 1024 x 1024 0.78 -> 0.80 ms).
+    const bool by_rows = s.mp % 128 == 0 && (long long)(s.mp / 128) * (s.mp / 128 + 1) / 2 * batch >= BIG_TILES;
+    if (!by_rows) X = nullptr;
     // workgroups per matrix: two pieces for each wavefront, up to what their joining costs
     const long long parts_l = ((long long)s.rows * ((s.cols + 255) / 256) + 7) / 8;
     const int parts = (int)(parts_l > NORM_PARTS ? NORM_PARTS : parts_l);
@@ -868,7 +885,7 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
     by_type(dtype, [&](auto *d) {
         using T = std::remove_pointer_t<decltype(d)>;
         hipLaunchKernelGGL((k_norm<T>), dim3(parts, batch), dim3(256), 0, st, p, s, parts, sums);
-        hipLaunchKernelGGL((k_split<T>), dim3((cp + 63) / 64, (rp + 63) / 64, batch), dim3(256), 0, st, p, s, parts, (const double *)sums, XT);
+        hipLaunchKernelGGL((k_split<T>), dim3((cp + 63) / 64, (rp + 63) / 64, batch), dim3(256), 0, st, p, s, parts, (const double *)sums, XT, X);
     });
     const auto two = [](int e) { return ldexpf(1.f, e); };
     const int pm = s.mp * 4;
@@ -897,16 +914,16 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
         char *A = mm[0], *T = mm[1], *Q = mm[2], *W = mm[3], *V = mm[4];
         {
             Gemm g = {};
-            g.A = g.B = XT;
+            g.A = g.B = by_rows ? X : XT;
             g.sA = g.sB = pl.x;
-            g.pitchA = g.pitchB = pm;
+            g.pitchA = g.pitchB = by_rows ? s.np * 4 : pm;
             g.K = s.np;
             g.symmetric = 1;
             g.alpha = two(EXP_A - 2 * EXP_X);
             g.sD = pl.mm;
             g.pitchD = pm;
             g.D = A;
-            gemm(g, s.mp, s.mp, true, batch, dtype, p, s, st);
+            gemm(g, s.mp, s.mp, !by_rows, batch, dtype, p, s, st);
         }
         const auto poly = [&](char *out) { // a I + b A + c A^2
             square(A, EXP_A, A, EXP_A, out, EXP_Q, NS_C, A, NS_B * two(EXP_Q - EXP_A), NS_A * two(EXP_Q));
@@ -941,6 +958,8 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
             g.sD = pl.x;
             g.D = YT;
             g.pitchD = pm;
+            g.M = X; // (not read by this product)
+            g.pitchM = s.np * 4;
         }
         gemm(g, s.mp, s.np, false, batch, dtype, p, s, st);
         char *t = XT;
