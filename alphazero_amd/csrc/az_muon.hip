@@ -31,6 +31,7 @@ constexpr int EXP_X = 15, EXP_A = 14, EXP_Q = 10; // stored number = value * 2^E
 constexpr int MAX_TABLE = 64;                     // matrices per launch when their addresses travel as kernel arguments
 constexpr int MAX_BATCH = 4096;                   // and at most
 constexpr int BIG_TILES = 256;                    // 128 x 128 tiles from this number of them on: one for every CU
+constexpr int FEW_TILES = 256;                    // up to here a CU has one workgroup at most
 constexpr int NORM_PARTS = 512;                   // partial sums of squares per matrix, at most
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -168,6 +169,8 @@ struct Gemm {
     const char *A2, *B2; // a second product of the same shape in the same launch (no E), or NULL
     char *D2;
     int batch;
+    int split;          // workgroups that share the K of a tile; their sums go to `parts`, 64 x 64 float32 each (k_join)
+    float *parts;
     char *M;            // the packed result by rows too, [M][N], or NULL
     int pitchM;
     char *D;            // packed result, by columns: [N][M]; NULL: to p.out() as G (columns: n, rows: m)
@@ -314,12 +317,14 @@ __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs
     const int group = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     char *lds = lds_all + group * 2 * STAGE;
     // workgroups go round the 8 XCDs: each XCD gets a run of neighbouring tiles, which share operands in its L2
-    int b, ti, tj;
+    int item, share, b, ti, tj;
     {
         const int n = gridDim.x, x = blockIdx.x & 7, i = blockIdx.x >> 3, per = n >> 3, rest = n & 7;
-        const int item = x * per + min(x, rest) + i;
-        b = item / a.tiles;
-        tile_at(item - b * a.tiles, a, ti, tj);
+        item = x * per + min(x, rest) + i;
+        const int whole = TURN ? item / a.split : item;
+        share = TURN ? item - whole * a.split : 0;
+        b = whole / a.tiles;
+        tile_at(whole - b * a.tiles, a, ti, tj);
     }
     if (a.D2 && b >= a.batch) {
         a.A = a.A2;
@@ -374,7 +379,13 @@ __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs
             for (int e = 0; e < 16; e++) acc[i][j][e] = low[i][j][e] = 0.f;
     const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
     const int lr = lane & 31, half = lane >> 5;
-    const int stages = a.K / BK;
+    int stages = a.K / BK;
+    if (TURN && a.split > 1) { // this workgroup's share of them
+        const int each = (stages + a.split - 1) / a.split, first = share * each;
+        stages = max(0, min(each, stages - first));
+#pragma unroll
+        for (int l = 0; l < LOADS; l++) src[l] += (size_t)first * (l * 4 < BM / 8 ? next_a : next_b);
+    }
     if (group < stages) load_stage(group, lds);
     const int rounds = (stages + KS - 1) / KS;
     for (int k = 0; k < rounds; k++) {
@@ -457,7 +468,39 @@ __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs
         }
         __syncthreads();
     }
+    if (TURN && a.split > 1) {
+        for (int e = threadIdx.x; e < BM * BN / 4; e += 256 * KS)
+            ((float4 *)(a.parts + (size_t)item * BM * BN))[e] = *(const float4 *)(t + tile_place<BM>(e % (BM / 4) * 4, e / (BM / 4)));
+        return;
+    }
     store_tile<BM, BN, 256 * KS, T>(t, a, p, s, b, ti, tj);
+}
+
+// a 64 x 64 tile from the sums of the workgroups that shared it, in their order
+__global__ __launch_bounds__(256) void k_join(Gemm a, Ptrs p, Shape s)
+{
+    __shared__ __align__(16) float t[64 * 68];
+    const int b = blockIdx.x / a.tiles;
+    int ti, tj;
+    tile_at(blockIdx.x - b * a.tiles, a, ti, tj);
+    const float4 *part = (const float4 *)(a.parts + (size_t)blockIdx.x * a.split * 64 * 64);
+    float4 v[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) v[q] = part[q * 256 + threadIdx.x];
+    for (int i = 1; i < a.split; i++) {
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const float4 o = part[(size_t)i * 1024 + q * 256 + threadIdx.x];
+            v[q].x += o.x; v[q].y += o.y; v[q].z += o.z; v[q].w += o.w;
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const int e = q * 256 + threadIdx.x;
+        *(float4 *)(t + tile_place<64>(e % 16 * 4, e / 16)) = v[q];
+    }
+    __syncthreads();
+    store_tile<64, 64, 256, float>(t, a, p, s, b, ti, tj);
 }
 
 // ---------------------------------------------------------------- small matrices: all steps in one launch
@@ -795,7 +838,7 @@ Shape shape_of(int rows, int cols)
 
 struct Plan {
     size_t x, mm;     // bytes of a packed X and of a packed m x m matrix
-    size_t sums, total;
+    size_t sums, parts, total;
 };
 Plan plan_of(const Shape &s, int batch)
 {
@@ -803,7 +846,8 @@ Plan plan_of(const Shape &s, int batch)
     p.x = (size_t)s.mp * s.np * 4;
     p.mm = (size_t)s.mp * s.mp * 4;
     p.sums = (size_t)batch * NORM_PARTS * sizeof(double);
-    p.total = p.sums + batch * (3 * p.x + 5 * p.mm);
+    p.parts = (size_t)FEW_TILES * 64 * 64 * 4;
+    p.total = p.sums + p.parts + batch * (3 * p.x + 5 * p.mm);
     return p;
 }
 
@@ -821,8 +865,17 @@ void gemm(Gemm a, int M, int N, bool turn, int batch, int dtype, const Ptrs &p, 
     a.tiles_m = M / t;
     a.tiles_n = N / t;
     // workgroups that leave CUs with one or two of them get more wavefronts each
-    const int ks = big ? 1 : groups <= 256 ? 4 : groups <= 512 ? 2 : 1;
-    const dim3 grid((unsigned)groups), block(256 * ks);
+    const int ks = big ? 1 : groups <= FEW_TILES ? 4 : groups <= 2 * FEW_TILES ? 2 : 1;
+    // Gram matrices of few tiles and a long K: a round of a workgroup (KS stages) takes about 1 us, joining the shares of
+    // several workgroups 4.5 us
+    a.split = 1;
+    if (turn && ks == 4) {
+        const int rounds = (a.K / BK + 3) / 4;
+        int most = (int)(FEW_TILES / groups);
+        if (most > (rounds + 1) / 2) most = (rounds + 1) / 2;
+        if (most > 1 && rounds - (rounds + most - 1) / most >= 6) a.split = most;
+    }
+    const dim3 grid((unsigned)(groups * a.split)), block(256 * ks);
     const auto go = [&](auto *kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, a, p, s); };
     const auto run = [&](auto turn, auto *d) {
         using T = std::remove_pointer_t<decltype(d)>;
@@ -832,7 +885,10 @@ void gemm(Gemm a, int M, int N, bool turn, int batch, int dtype, const Ptrs &p, 
         else if (ks == 2) go(k_gemm<64, 64, 2, TURN, T>);
         else go(k_gemm<64, 64, 1, TURN, T>);
     };
-    if (turn) run(std::true_type(), (float *)nullptr);
+    if (turn) {
+        run(std::true_type(), (float *)nullptr);
+        if (a.split > 1) hipLaunchKernelGGL(k_join, dim3((unsigned)groups), dim3(256), 0, st, a, p, s);
+    }
     else if (a.D) run(std::false_type(), (float *)nullptr);
     else by_type(dtype, [&](auto *d) { run(std::false_type(), d); });
 }
@@ -870,7 +926,8 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
 {
     const Plan pl = plan_of(s, batch);
     double *sums = (double *)work;
-    char *XT = work + pl.sums, *YT = XT + batch * pl.x, *X = YT + batch * pl.x;
+    float *parts_at = (float *)(work + pl.sums);
+    char *XT = work + pl.sums + pl.parts, *YT = XT + batch * pl.x, *X = YT + batch * pl.x;
     char *mm[5];
     for (int i = 0; i < 5; i++) mm[i] = X + batch * pl.x + i * batch * pl.mm;
     // Transposing LDS reads are half as fast as plain ones.  That does not matter where loads are waited for, but a Gram
@@ -923,6 +980,7 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
             g.sD = pl.mm;
             g.pitchD = pm;
             g.D = A;
+            g.parts = parts_at;
             gemm(g, s.mp, s.mp, !by_rows, batch, dtype, p, s, st);
         }
         const auto poly = [&](char *out) { // a I + b A + c A^2
