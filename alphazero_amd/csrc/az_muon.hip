@@ -171,6 +171,7 @@ struct Gemm {
     int batch;
     int split;          // workgroups that share the K of a tile; their sums go to `parts`, 64 x 64 float32 each (k_join)
     float *parts;
+    int poly;           // the tile is the whole matrix and D is to hold Q (k_join_poly)
     char *M;            // the packed result by rows too, [M][N], or NULL
     int pitchM;
     char *D;            // packed result, by columns: [N][M]; NULL: to p.out() as G (columns: n, rows: m)
@@ -380,7 +381,7 @@ __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs
     const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
     const int lr = lane & 31, half = lane >> 5;
     int stages = a.K / BK;
-    if (TURN && a.split > 1) { // this workgroup's share of them
+    if (TURN && a.parts) { // this workgroup's share of them
         const int each = (stages + a.split - 1) / a.split, first = share * each;
         stages = max(0, min(each, stages - first));
 #pragma unroll
@@ -468,13 +469,63 @@ __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs
         }
         __syncthreads();
     }
-    if (TURN && a.split > 1) {
+    if (TURN && a.parts) {
         for (int e = threadIdx.x; e < BM * BN / 4; e += 256 * KS)
             ((float4 *)(a.parts + (size_t)item * BM * BN))[e] = *(const float4 *)(t + tile_place<BM>(e % (BM / 4) * 4, e / (BM / 4)));
         return;
     }
     store_tile<BM, BN, 256 * KS, T>(t, a, p, s, b, ti, tj);
 }
+
+// 16-byte piece of a row of M * 4 bytes: rows spread over the banks
+template <int M> __device__ __forceinline__ int bank(int r, int piece) { return M == 64 ? piece ^ (r & 15) : piece ^ ((r >> 1) & 7); }
+// first of the two pieces (hi, lo) of the 8 columns 16 c + 4 h + {0..3, 8..11} of a packed row
+__device__ __forceinline__ int slot(int c, int h) { return (c * 2 + h) * 2; }
+
+__device__ __forceinline__ void split8(const float *v, h8 &hi, h8 &lo)
+{
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        hi[i] = (_Float16)v[i];
+        lo[i] = (_Float16)fmaf(-1.f, (float)hi[i], v[i]); // exact (one instruction: an operand may be float16)
+    }
+}
+
+// A tile (rows 32 i, columns 32 j) of Q = a I + b A + c A^2, times 2^EXP_Q, for A of M x M in LDS (rows of blocks of 16
+// columns, in a block the 8 of slot 0, then of slot 1, hi and lo).  A lane's results are four rows side by side of its
+// column, so (Q is symmetric) f[c] is what slot `half` of block 2 i + c of row 32 j + lane mod 32 holds, and the elements of
+// A that go with it stand in the same place.
+template <int M> __device__ __forceinline__ void poly_tile(const char *sA, int i, int j, int lane, float (&f)[2][8])
+{
+    constexpr int C = M / 16;
+    const int lr = lane & 31, half = lane >> 5, ra = i * 32 + lr, rb = j * 32 + lr;
+    f16v acc;
+#pragma unroll
+    for (int e = 0; e < 16; e++) acc[e] = 0.f;
+    h8 ah[C], bh[C];
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        ah[c] = *(const h8 *)(sA + ra * M * 4 + bank<M>(ra, slot(c, half)) * 16);
+        bh[c] = *(const h8 *)(sA + rb * M * 4 + bank<M>(rb, slot(c, half)) * 16);
+        const h8 al = *(const h8 *)(sA + ra * M * 4 + bank<M>(ra, slot(c, half) + 1) * 16);
+        const h8 bl = *(const h8 *)(sA + rb * M * 4 + bank<M>(rb, slot(c, half) + 1) * 16);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh[c], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[c], bl, acc, 0, 0, 0);
+    }
+#pragma unroll
+    for (int c = 0; c < C; c++) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[c], bh[c], acc, 0, 0, 0);
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+        const char *at = sA + rb * M * 4;
+        const h8 hi = *(const h8 *)(at + bank<M>(rb, slot(2 * i + c, half)) * 16), lo = *(const h8 *)(at + bank<M>(rb, slot(2 * i + c, half) + 1) * 16);
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            f[c][k] = fmaf((float)hi[k] + (float)lo[k], NS_B * 0x1p-4f, acc[8 * c + k] * (NS_C * 0x1p-18f)); // 2^(EXP_Q - EXP_A), 2^(EXP_Q - 2 EXP_A)
+            if (i * 32 + 16 * c + 8 * (k >> 2) + 4 * half + (k & 3) == rb) f[c][k] += NS_A * 0x1p10f;
+        }
+    }
+}
+static_assert(EXP_X == 15 && EXP_A == 14 && EXP_Q == 10, "the powers of two written out in poly_tile and k_small");
 
 // a 64 x 64 tile from the sums of the workgroups that shared it, in their order
 __global__ __launch_bounds__(256) void k_join(Gemm a, Ptrs p, Shape s)
@@ -503,6 +554,59 @@ __global__ __launch_bounds__(256) void k_join(Gemm a, Ptrs p, Shape s)
     store_tile<64, 64, 256, float>(t, a, p, s, b, ti, tj);
 }
 
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+
+// The same where the tile is the whole Gram matrix (up to 64 rows), and Q at once, packed to a.D: one launch less a step
+__global__ __launch_bounds__(256) void k_join_poly(Gemm a)
+{
+    __shared__ __align__(16) char sA[64 * 256];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const float4 *part = (const float4 *)(a.parts + (size_t)blockIdx.x * a.split * 64 * 64);
+    float4 v[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) v[q] = part[q * 256 + threadIdx.x];
+    for (int i = 1; i < a.split; i++) {
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const float4 o = part[(size_t)i * 1024 + q * 256 + threadIdx.x];
+            v[q].x += o.x; v[q].y += o.y; v[q].z += o.z; v[q].w += o.w;
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const int e = q * 256 + threadIdx.x, r = e % 16 * 4, c = e / 16; // rows r..r+3 of column c, stored as row c
+        const float x[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+        h4 hi, lo;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            hi[k] = (_Float16)x[k];
+            lo[k] = (_Float16)fmaf(-1.f, (float)hi[k], x[k]);
+        }
+        char *row = sA + c * 256 + (r >> 3 & 1) * 8;
+        *(h4 *)(row + bank<64>(c, slot(r >> 4, r >> 2 & 1)) * 16) = hi;
+        *(h4 *)(row + bank<64>(c, slot(r >> 4, r >> 2 & 1) + 1) * 16) = lo;
+    }
+    __syncthreads();
+    const int i = wave >> 1, j = wave & 1, half = lane >> 5;
+    float f[2][8];
+    poly_tile<64>(sA, i, j, lane, f);
+    char *D = a.D + blockIdx.x * a.sD + (size_t)(j * 32 + (lane & 31)) * a.pitchD;
+#pragma unroll
+    for (int c = 0; c < 2; c++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) { // columns 16 (2 i + c) + 8 u + 4 half + {0..3}
+            h4 hi, lo;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                hi[k] = (_Float16)f[c][4 * u + k];
+                lo[k] = (_Float16)fmaf(-1.f, (float)hi[k], f[c][4 * u + k]);
+            }
+            char *at = D + (16 * (2 * i + c) + 8 * u) * 4 + 4 * half * 2;
+            *(h4 *)at = hi;
+            *(h4 *)(at + 16) = lo;
+        }
+}
+
 // ---------------------------------------------------------------- small matrices: all steps in one launch
 //
 // A matrix of m <= 32 MT rows and n <= 256 NT columns belongs to one workgroup of 8 wavefronts and stays in registers:
@@ -513,20 +617,6 @@ __global__ __launch_bounds__(256) void k_join(Gemm a, Ptrs p, Shape s)
 // (17 of them, 5 us each); this one is bound by the latency of 3 barriers a step (2 up to 32 rows) and
 // by one CU's matrix cores and its share of the memory (11 of 40 us at 64 x 576 go into reading and writing).
 constexpr int SMALL_WAVES = 8;
-
-// 16-byte piece of a row of M * 4 bytes: rows spread over the banks
-template <int M> __device__ __forceinline__ int bank(int r, int piece) { return M == 64 ? piece ^ (r & 15) : piece ^ ((r >> 1) & 7); }
-// first of the two pieces (hi, lo) of the 8 columns 16 c + 4 h + {0..3, 8..11} of a packed row
-__device__ __forceinline__ int slot(int c, int h) { return (c * 2 + h) * 2; }
-
-__device__ __forceinline__ void split8(const float *v, h8 &hi, h8 &lo)
-{
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        hi[i] = (_Float16)v[i];
-        lo[i] = (_Float16)fmaf(-1.f, (float)hi[i], v[i]); // exact (one instruction: an operand may be float16)
-    }
-}
 
 __device__ __forceinline__ int row_of(int r) { return (r & ~12) | (r & 4) << 1 | (r & 8) >> 1; }
 
@@ -694,38 +784,15 @@ template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES
             *(h8 *)(sA + r * M * 4 + bank<M>(r, slot(c16, h) + 1) * 16) = lo;
         }
         __syncthreads();
-        // Q = a I + b A + c A^2: one 32 x 32 tile per wavefront, or the only tile in every one.  A lane's results are four
-        // rows side by side of its column, so (Q is symmetric) the 8 of a block are an operand's share of row `rb`, and
-        // so are the elements of A that go with them.
+        // one 32 x 32 tile of Q per wavefront, or the only one in every wavefront
         h8 qh1[2], ql1[2];
         if (MT == 1 ? wave < tiles : wave < MT * MT) {
-            const int i = MT == 1 ? 0 : wave / MT, j = MT == 1 ? 0 : wave % MT, ra = i * 32 + lr, rb = j * 32 + lr;
-            f16v acc;
-#pragma unroll
-            for (int e = 0; e < 16; e++) acc[e] = 0.f;
-            h8 ah[C], bh[C];
-#pragma unroll
-            for (int c = 0; c < C; c++) {
-                ah[c] = *(const h8 *)(sA + ra * M * 4 + bank<M>(ra, slot(c, half)) * 16);
-                bh[c] = *(const h8 *)(sA + rb * M * 4 + bank<M>(rb, slot(c, half)) * 16);
-                const h8 al = *(const h8 *)(sA + ra * M * 4 + bank<M>(ra, slot(c, half) + 1) * 16);
-                const h8 bl = *(const h8 *)(sA + rb * M * 4 + bank<M>(rb, slot(c, half) + 1) * 16);
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh[c], acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[c], bl, acc, 0, 0, 0);
-            }
-#pragma unroll
-            for (int c = 0; c < C; c++) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[c], bh[c], acc, 0, 0, 0);
+            const int i = MT == 1 ? 0 : wave / MT, j = MT == 1 ? 0 : wave % MT, rb = j * 32 + lr;
+            float f[2][8];
+            poly_tile<M>(sA, i, j, lane, f);
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                const char *at = sA + rb * M * 4;
-                const h8 hi = *(const h8 *)(at + bank<M>(rb, slot(2 * i + c, half)) * 16), lo = *(const h8 *)(at + bank<M>(rb, slot(2 * i + c, half) + 1) * 16);
-                float f[8];
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    f[k] = fmaf((float)hi[k] + (float)lo[k], NS_B * 0x1p-4f, acc[8 * c + k] * (NS_C * 0x1p-18f)); // 2^(EXP_Q - EXP_A), 2^(EXP_Q - 2 EXP_A)
-                    if (i * 32 + 16 * c + 8 * (k >> 2) + 4 * half + (k & 3) == rb) f[k] += NS_A * 0x1p10f;
-                }
-                split8(f, qh1[c], ql1[c]);
+                split8(f[c], qh1[c], ql1[c]);
                 if (MT > 1) {
                     *(h8 *)(sQ + rb * M * 4 + bank<M>(rb, slot(2 * i + c, half)) * 16) = qh1[c];
                     *(h8 *)(sQ + rb * M * 4 + bank<M>(rb, slot(2 * i + c, half) + 1) * 16) = ql1[c];
@@ -808,7 +875,6 @@ template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES
     } else if (s.m == M) store(std::true_type());
     else store(std::false_type());
 }
-static_assert(EXP_X == 15 && EXP_A == 14 && EXP_Q == 10, "the powers of two written out in k_small");
 
 // ---------------------------------------------------------------- host side
 
@@ -874,7 +940,9 @@ void gemm(Gemm a, int M, int N, bool turn, int batch, int dtype, const Ptrs &p, 
         int most = (int)(FEW_TILES / groups);
         if (most > (rounds + 1) / 2) most = (rounds + 1) / 2;
         if (most > 1 && rounds - (rounds + most - 1) / most >= 6) a.split = most;
+        if (a.poly) a.split = most;
     }
+    if (a.split == 1 && !a.poly) a.parts = nullptr;
     const dim3 grid((unsigned)(groups * a.split)), block(256 * ks);
     const auto go = [&](auto *kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, a, p, s); };
     const auto run = [&](auto turn, auto *d) {
@@ -887,7 +955,8 @@ void gemm(Gemm a, int M, int N, bool turn, int batch, int dtype, const Ptrs &p, 
     };
     if (turn) {
         run(std::true_type(), (float *)nullptr);
-        if (a.split > 1) hipLaunchKernelGGL(k_join, dim3((unsigned)groups), dim3(256), 0, st, a, p, s);
+        if (a.poly) hipLaunchKernelGGL(k_join_poly, dim3((unsigned)groups), dim3(256), 0, st, a);
+        else if (a.parts) hipLaunchKernelGGL(k_join, dim3((unsigned)groups), dim3(256), 0, st, a, p, s);
     }
     else if (a.D) run(std::false_type(), (float *)nullptr);
     else by_type(dtype, [&](auto *d) { run(std::false_type(), d); });
@@ -964,7 +1033,9 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
     // Steps per group.  float32 results take every step on X (the error stays at or below that of float32 products).
     // Results of 16 bits (half a step: 2^-9, 2^-12) have room for three, which pay as soon as X is wider than high: of five
     // steps' 27.5 m^3 products at n = 1.5 m 23 are left, of 65 at n = 4 m 38.
-    const int group = dtype != AZ_F32 && 2 * s.n >= 3 * s.m ? 3 : 1;
+    // Up to 64 rows a step is three launches, whatever it computes: the Gram matrix, its joining with Q, the product.
+    const bool at_once = s.mp == 64 && batch <= FEW_TILES;
+    const int group = !at_once && dtype != AZ_F32 && 2 * s.n >= 3 * s.m ? 3 : 1;
     for (int left = steps; left > 0;) {
         // (the odd ones first: the longer groups start from the better conditioned matrix)
         const int k = left > group ? (left % group ? left % group : group) : left;
@@ -979,7 +1050,8 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
             g.alpha = two(EXP_A - 2 * EXP_X);
             g.sD = pl.mm;
             g.pitchD = pm;
-            g.D = A;
+            g.poly = at_once;
+            g.D = at_once ? W : A;
             g.parts = parts_at;
             gemm(g, s.mp, s.mp, !by_rows, batch, dtype, p, s, st);
         }
@@ -987,7 +1059,7 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
             square(A, EXP_A, A, EXP_A, out, EXP_Q, NS_C, A, NS_B * two(EXP_Q - EXP_A), NS_A * two(EXP_Q));
         };
         // W, V: Q of the group's latest steps; the product of all of them ends in `total`
-        poly(W);
+        if (!at_once) poly(W);
         const char *total = W;
         if (k > 1) {
             square(A, EXP_A, W, EXP_Q, T, EXP_A);

@@ -72,6 +72,18 @@ def test_numbers_of_steps(steps, shape):
         assert 0.6 < s.min() and s.max() < 1.25
 
 
+@pytest.mark.parametrize("shape", [(3, 64, 2304), (4608, 20), (300, 4000), (2, 129, 3000), (300, 33, 800), (2, 1500, 40), (1, 1050, 1400)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_gram_sums_and_large_tiles(shape, dtype):
+    # K shared by several workgroups, with Q at once up to 64 rows, more matrices than CUs; tiles of 128
+    from alphazero_amd import muon
+
+    g = _updates(shape, 4).to(dtype).cuda()
+    got = muon.orthogonalise(g)
+    _check(got, g)
+    assert torch.equal(got, muon.orthogonalise(g))
+
+
 @pytest.mark.parametrize("count", [1, 2, 7, 63, 64, 65, 130])
 def test_batches(count):
     from alphazero_amd import muon
