@@ -105,10 +105,11 @@ def test_low_rank_sizes_and_zeros(shape):
     got = muon.orthogonalise(g)
     assert not got[0].any() and torch.isfinite(got).all()
     if shape[0] > 1:
-        g[1, 3, 5] = math.nan
-        got = muon.orthogonalise(g)
-        assert got[1].isnan().all() and not got[0].any()
-        assert shape[0] < 3 or torch.isfinite(got[2]).all()
+        for bad in (math.nan, math.inf):
+            g[1, 3, 5] = bad
+            got = muon.orthogonalise(g)
+            assert got[1].isnan().all() and not got[0].any()
+            assert shape[0] < 3 or torch.isfinite(got[2]).all()
 
 
 def test_strides_lists_and_empty():
