@@ -590,7 +590,7 @@ template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_parts(Ro
         m = wave_max(m);
         if (m > M) {
             if (M != NINF) {
-                if (pi) X += W * (M - m);
+                if (pi) X += W == 0.f ? 0.f : W * (M - m);
                 rebase(S, U, M, m);
             }
             M = m;
@@ -855,7 +855,7 @@ int grid_of(long long units)
 // one step, at most as many as one wavefront can merge (their lists in 32 KB of LDS).
 Chunks chunks_of(int n, int A, int top)
 {
-    long long want = n > 0 ? (8192 + n - 1) / n : 1;
+    long long want = n > 0 ? (8192ll + n - 1) / n : 1;
     const long long most = (A + LONG_STEP - 1) / LONG_STEP;
     const long long fit = top > 16 ? MAX_CHUNKS / 2 : MAX_CHUNKS;
     if (want > most) want = most;

@@ -187,6 +187,26 @@ def test_special_values():
     assert abs(t.logp.item() + math.log1p(math.e)) < 1e-6
 
 
+def test_values_at_the_ends_of_the_range_in_long_rows():
+    # differences that leave float32's range, between chunks and between steps of a chunk
+    from alphazero_amd import policy
+
+    x = torch.full((2, 70000), -3e38, device="cuda")
+    x[0, 69999] = 3e38
+    x[1, 5], x[1, 40000], x[1, 3000] = 3e38, 3e38, -math.inf
+    pi = torch.zeros(2, 70000, device="cuda")
+    pi[0, 69999], pi[1, 5], pi[1, 40000] = 1.0, 0.5, 0.5
+    s = policy.score(x, torch.tensor([[69999, 0], [5, 3000]], device="cuda"), top=3)
+    assert s.top_moves.tolist() == [[69999, 0, 1], [5, 40000, 0]]
+    assert s.logp[0, 0] == 0 and s.logp[0, 1] == -math.inf and s.logp[1, 1] == -math.inf
+    assert abs(s.logp[1, 0].item() + math.log(2)) < 1e-6 and s.entropy[0] == 0 and abs(s.entropy[1].item() - math.log(2)) < 1e-6
+    x.requires_grad_()
+    v = torch.zeros(2, device="cuda")
+    total = policy.loss(x, v, pi, v)
+    d, = torch.autograd.grad(total, x)
+    assert abs(total.item()) < 1e-6 and not d.any()
+
+
 def _loss_inputs(rows, actions, dtype, mask, seed):
     x, legal = _inputs(rows, actions, dtype, mask, seed)
     g = torch.Generator().manual_seed(seed + 1)
