@@ -106,11 +106,17 @@ class Muon(torch.optim.Optimizer):
         if not isinstance(steps, int) or not 1 <= steps <= MAX_STEPS:
             _refuse(f"steps must be 1..{MAX_STEPS}")
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps))
-        for group in self.param_groups:
-            for p in group["params"]:
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        try:
+            for p in self.param_groups[-1]["params"]:
                 if p.dim() < 2:
                     _refuse("Muon takes weights of two or more dimensions")
-                _check(p.shape[0], p[0].numel() if p.shape[0] else 0, p.dtype, group["steps"])
+                _check(p.shape[0], p[0].numel() if p.shape[0] else 0, p.dtype, self.param_groups[-1]["steps"])
+        except ValueError:
+            self.param_groups.pop()
+            raise
 
     @staticmethod
     def weights_of(module):

@@ -51,3 +51,14 @@ def test_optimiser_refuses():
             muon.Muon([p], **kw)
     with pytest.raises(ValueError, match="two or more"):
         muon.Muon([torch.nn.Parameter(torch.zeros(3))])
+
+
+def test_optimiser_refuses_later_groups():
+    opt = muon.Muon([torch.nn.Parameter(torch.zeros(3, 3))])
+    for group in (dict(params=[torch.nn.Parameter(torch.zeros(3))]), dict(params=[torch.nn.Parameter(torch.zeros(2, 2))], steps=0),
+                  dict(params=[torch.nn.Parameter(torch.zeros(2, 2, dtype=torch.float64))])):
+        with pytest.raises(ValueError):
+            opt.add_param_group(group)
+        assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(2, 5))], lr=0.1))
+    assert len(opt.param_groups) == 2
