@@ -94,15 +94,21 @@ template <class T> __global__ __launch_bounds__(256) void k_norm(Ptrs p, Shape s
     if (threadIdx.x == 0) sums[(size_t)blockIdx.y * NORM_PARTS + blockIdx.x] = (s_w[0] + s_w[1]) + (s_w[2] + s_w[3]);
 }
 
-// hi and lo halves of 8 numbers, 32 bytes at p
+// hi and lo halves of a number.  It is hidden from the compiler how v came about: it may compute hi twice, once rounded
+// from v and once straight from the factors of a product (other bits next to a tie), and take lo from the other one.
+template <class V> __device__ __forceinline__ void split1(float v, V &hi, V &lo, int i)
+{
+    asm("" : "+v"(v));
+    hi[i] = (_Float16)v;
+    lo[i] = (_Float16)fmaf(-1.f, (float)hi[i], v); // exact (one instruction: an operand may be float16)
+}
+
+// of 8 numbers, 32 bytes at p
 __device__ __forceinline__ void pack8(char *p, const float (&v)[8])
 {
     h8 hi, lo;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        hi[i] = (_Float16)v[i];
-        lo[i] = (_Float16)fmaf(-1.f, (float)hi[i], v[i]);
-    }
+    for (int i = 0; i < 8; i++) split1(v[i], hi, lo, i);
     *(h8 *)p = hi;
     *(h8 *)(p + 16) = lo;
 }
@@ -485,10 +491,7 @@ __device__ __forceinline__ int slot(int c, int h) { return (c * 2 + h) * 2; }
 __device__ __forceinline__ void split8(const float *v, h8 &hi, h8 &lo)
 {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        hi[i] = (_Float16)v[i];
-        lo[i] = (_Float16)fmaf(-1.f, (float)hi[i], v[i]); // exact (one instruction: an operand may be float16)
-    }
+    for (int i = 0; i < 8; i++) split1(v[i], hi, lo, i);
 }
 
 // A tile (rows 32 i, columns 32 j) of Q = a I + b A + c A^2, times 2^EXP_Q, for A of M x M in LDS (rows of blocks of 16
@@ -578,10 +581,7 @@ __global__ __launch_bounds__(256) void k_join_poly(Gemm a)
         const float x[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
         h4 hi, lo;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            hi[k] = (_Float16)x[k];
-            lo[k] = (_Float16)fmaf(-1.f, (float)hi[k], x[k]);
-        }
+        for (int k = 0; k < 4; k++) split1(x[k], hi, lo, k);
         char *row = sA + c * 256 + (r >> 3 & 1) * 8;
         *(h4 *)(row + bank<64>(c, slot(r >> 4, r >> 2 & 1)) * 16) = hi;
         *(h4 *)(row + bank<64>(c, slot(r >> 4, r >> 2 & 1) + 1) * 16) = lo;
@@ -597,10 +597,7 @@ __global__ __launch_bounds__(256) void k_join_poly(Gemm a)
         for (int u = 0; u < 2; u++) { // columns 16 (2 i + c) + 8 u + 4 half + {0..3}
             h4 hi, lo;
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                hi[k] = (_Float16)f[c][4 * u + k];
-                lo[k] = (_Float16)fmaf(-1.f, (float)hi[k], f[c][4 * u + k]);
-            }
+            for (int k = 0; k < 4; k++) split1(f[c][4 * u + k], hi, lo, k);
             char *at = D + (16 * (2 * i + c) + 8 * u) * 4 + 4 * half * 2;
             *(h4 *)at = hi;
             *(h4 *)(at + 16) = lo;
@@ -691,7 +688,8 @@ template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES
 #pragma unroll
         for (int w = 0; w < SMALL_WAVES; w++) sum += ((double *)lds)[w];
         __syncthreads();
-        // 1 / |X| = f 2^k with f in [1/2, 1]: a float32 product, rounded once, and a power of two
+        // 1 / |X| = f 2^k with f in [1/2, 1]: the power of two first (the smallest float32 numbers lose nothing), then a
+        // float32 product, rounded once
         int k;
         const float f = sum == 0. ? 0.f : (float)frexp(1. / sqrt(sum), &k);
         k = sum == 0. ? 0 : k + EXP_X;
@@ -700,7 +698,7 @@ template <int MT, int NT, class T> __global__ __launch_bounds__(64 * SMALL_WAVES
 #pragma unroll
             for (int c = 0; c < C; c++) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) x[t][c][e] = ldexpf(x[t][c][e] * f, k);
+                for (int e = 0; e < 8; e++) x[t][c][e] = ldexpf(x[t][c][e], k) * f;
                 split8(x[t][c], xh[t][c], xl[t][c]);
             }
     }

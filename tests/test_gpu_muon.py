@@ -112,6 +112,29 @@ def test_low_rank_sizes_and_zeros(shape):
             assert shape[0] < 3 or torch.isfinite(got[2]).all()
 
 
+@pytest.mark.parametrize("shape", [(8, 16, 144), (8, 30, 600), (8, 64, 576), (2, 64, 4000), (2, 128, 1024), (1, 500, 2048)])
+def test_every_number_of_wide_matrices_has_float32_precision(shape):
+    # The singular values of a wide random matrix lie close together, so no direction's error outgrows the others: five
+    # steps of at most 8 u each (the bound above) and as much again for their mutual growth are 80 u.  One number of X or Q
+    # kept to 11 bits instead of 22 would show: 2^-12 / sqrt(m n) of X, of many more where several are.
+    from alphazero_amd import muon
+
+    g = _updates(shape, 21)
+    off = muon.orthogonalise(g.cuda()).cpu().double() - _exact(g)
+    assert (off.flatten(-2).norm(dim=-1) <= 80 * U * _exact(g).flatten(-2).norm(dim=-1)).all()
+
+
+@pytest.mark.parametrize("shape", [(5, 9), (48, 100), (100, 200)])
+def test_the_smallest_numbers(shape):
+    # subnormal float32 numbers: whole multiples of 2^-149
+    from alphazero_amd import muon
+
+    gen = torch.Generator().manual_seed(8)
+    g = torch.ldexp(torch.randint(-300, 301, shape, generator=gen).float(), torch.tensor(-120)) * 2.0 ** -29
+    assert 0 < g.abs().max() < 2.0 ** -126
+    _check(muon.orthogonalise(g.cuda()), g)
+
+
 def test_strides_lists_and_empty():
     from alphazero_amd import muon
 
