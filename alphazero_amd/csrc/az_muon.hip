@@ -30,8 +30,9 @@ constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr int EXP_X = 15, EXP_A = 14, EXP_Q = 10; // stored number = value * 2^EXP
 constexpr int MAX_TABLE = 64;                     // matrices per launch when their addresses travel as kernel arguments
 constexpr int MAX_BATCH = 4096;                   // and at most
-constexpr int BIG_TILES = 256;                    // 128 x 128 tiles from this number of them on: one for every CU
-constexpr int FEW_TILES = 256;                    // up to here a CU has one workgroup at most
+constexpr int CUS = 256;
+constexpr int BIG_TILES = 192;                    // 128 x 128 tiles from this number of them on
+constexpr int FEW_TILES = CUS;                    // up to here a CU has one workgroup at most
 constexpr int NORM_PARTS = 512;                   // partial sums of squares per matrix, at most
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -175,7 +176,8 @@ struct Gemm {
     const char *A2, *B2; // a second product of the same shape in the same launch (no E), or NULL
     char *D2;
     int batch;
-    int split;          // workgroups that share the K of a tile; their sums go to `parts`, 64 x 64 float32 each (k_join)
+    int whole;          // tiles (of all matrices) with a workgroup of their own; of the others ...
+    int split;          // ... so many workgroups share the K of each, their float32 sums go to `parts` (k_join)
     float *parts;
     int poly;           // the tile is the whole matrix and D is to hold Q (k_join_poly)
     char *M;            // the packed result by rows too, [M][N], or NULL
@@ -311,7 +313,9 @@ __device__ __forceinline__ void store_tile(float *t, const Gemm &a, const Ptrs &
 // KS groups of 4 wavefronts take every KS-th stage of K, each with stages of its own, and add up at the end: where tiles
 // are few a CU needs more loads in flight (what one asks for arrives after 2100 cycles).  Measured with one group /
 // four: 256 x 2304, one matrix 225 / 174 us, 4 x 512 x 512 191 / 153 us.  (Every wavefront on its own, a whole tile each,
-// with four pieces of K in flight: 200 and 173 us.)
+// with four pieces of K in flight: 200 and 173 us.)  Large tiles: a CU that has one workgroup of two groups is busy, with
+// one of one group it waits (210 symmetric tiles, K = 2560: 60 us; as 820 tiles of 64, four to a CU: 82 us).
+// The last tiles may be shared: workgroups take parts of their K and leave float32 sums for k_join.
 // TURN: A and B are given as [K][M] and [K][N] (the Gram matrix from X'), and the LDS reads transpose.
 template <int BM, int BN, int KS, bool TURN, class T>
 __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs p, Shape s)
@@ -323,15 +327,22 @@ __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
     const int group = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     char *lds = lds_all + group * 2 * STAGE;
+    constexpr bool SHARES = BM == 64 ? TURN && KS == 4 : KS == 2; // some tiles may be shared
     // workgroups go round the 8 XCDs: each XCD gets a run of neighbouring tiles, which share operands in its L2
-    int item, share, b, ti, tj;
+    int item, share = -1, b, ti, tj;
     {
-        const int n = gridDim.x, x = blockIdx.x & 7, i = blockIdx.x >> 3, per = n >> 3, rest = n & 7;
+        const bool shared = SHARES && (int)blockIdx.x >= a.whole; // (of the workgroups behind `whole` each XCD gets a run too)
+        const int at = shared ? blockIdx.x - a.whole : blockIdx.x, n = shared ? gridDim.x - a.whole : SHARES ? a.whole : gridDim.x;
+        const int x = at & 7, i = at >> 3, per = n >> 3, rest = n & 7;
         item = x * per + min(x, rest) + i;
-        const int whole = TURN ? item / a.split : item;
-        share = TURN ? item - whole * a.split : 0;
-        b = whole / a.tiles;
-        tile_at(whole - b * a.tiles, a, ti, tj);
+        int tile = item;
+        if (shared) {
+            tile = item / a.split;
+            share = item - tile * a.split;
+            tile += a.whole;
+        }
+        b = tile / a.tiles;
+        tile_at(tile - b * a.tiles, a, ti, tj);
     }
     if (a.D2 && b >= a.batch) {
         a.A = a.A2;
@@ -387,7 +398,7 @@ __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs
     const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
     const int lr = lane & 31, half = lane >> 5;
     int stages = a.K / BK;
-    if (TURN && a.parts) { // this workgroup's share of them
+    if (SHARES && share >= 0) { // this workgroup's share of them
         const int each = (stages + a.split - 1) / a.split, first = share * each;
         stages = max(0, min(each, stages - first));
 #pragma unroll
@@ -475,7 +486,7 @@ __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs
         }
         __syncthreads();
     }
-    if (TURN && a.parts) {
+    if (SHARES && share >= 0) {
         for (int e = threadIdx.x; e < BM * BN / 4; e += 256 * KS)
             ((float4 *)(a.parts + (size_t)item * BM * BN))[e] = *(const float4 *)(t + tile_place<BM>(e % (BM / 4) * 4, e / (BM / 4)));
         return;
@@ -530,22 +541,30 @@ template <int M> __device__ __forceinline__ void poly_tile(const char *sA, int i
 }
 static_assert(EXP_X == 15 && EXP_A == 14 && EXP_Q == 10, "the powers of two written out in poly_tile and k_small");
 
-// a 64 x 64 tile from the sums of the workgroups that shared it, in their order
-__global__ __launch_bounds__(256) void k_join(Gemm a, Ptrs p, Shape s)
+// the sums of the workgroups that shared a tile, in their order; 64 x 64 of its results per workgroup
+template <int BM, class T> __global__ __launch_bounds__(256) void k_join(Gemm a, Ptrs p, Shape s)
 {
+    constexpr int Q = BM / 64;
     __shared__ __align__(16) float t[64 * 68];
-    const int b = blockIdx.x / a.tiles;
-    int ti, tj;
-    tile_at(blockIdx.x - b * a.tiles, a, ti, tj);
-    const float4 *part = (const float4 *)(a.parts + (size_t)blockIdx.x * a.split * 64 * 64);
+    const int tile = blockIdx.x / (Q * Q), q_row = blockIdx.x % Q, q_col = blockIdx.x / Q % Q;
+    int b = (a.whole + tile) / a.tiles, ti, tj;
+    tile_at(a.whole + tile - b * a.tiles, a, ti, tj);
+    if (a.D2 && b >= a.batch) {
+        a.D = a.D2;
+        b -= a.batch;
+    }
+    if (a.symmetric && ti == tj && q_row > q_col) return; // (written with its mirror image)
+    const float *part = a.parts + (size_t)tile * a.split * BM * BM + q_col * 64 * BM + q_row * 64;
     float4 v[4];
-#pragma unroll
-    for (int q = 0; q < 4; q++) v[q] = part[q * 256 + threadIdx.x];
-    for (int i = 1; i < a.split; i++) {
+    for (int i = 0; i < a.split; i++) {
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-            const float4 o = part[(size_t)i * 1024 + q * 256 + threadIdx.x];
-            v[q].x += o.x; v[q].y += o.y; v[q].z += o.z; v[q].w += o.w;
+            const int e = q * 256 + threadIdx.x;
+            const float4 o = *(const float4 *)(part + (size_t)i * BM * BM + e / 16 * BM + e % 16 * 4);
+            if (i == 0) v[q] = o;
+            else {
+                v[q].x += o.x; v[q].y += o.y; v[q].z += o.z; v[q].w += o.w;
+            }
         }
     }
 #pragma unroll
@@ -554,7 +573,7 @@ __global__ __launch_bounds__(256) void k_join(Gemm a, Ptrs p, Shape s)
         *(float4 *)(t + tile_place<64>(e % 16 * 4, e / 16)) = v[q];
     }
     __syncthreads();
-    store_tile<64, 64, 256, float>(t, a, p, s, b, ti, tj);
+    store_tile<64, 64, 256, T>(t, a, p, s, b, ti * Q + q_row, tj * Q + q_col);
 }
 
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
@@ -910,7 +929,7 @@ Plan plan_of(const Shape &s, int batch)
     p.x = (size_t)s.mp * s.np * 4;
     p.mm = (size_t)s.mp * s.mp * 4;
     p.sums = (size_t)batch * NORM_PARTS * sizeof(double);
-    p.parts = (size_t)FEW_TILES * 64 * 64 * 4;
+    p.parts = (size_t)CUS * 128 * 128 * 4; // sums of shared tiles: at most a large one for every CU
     p.total = p.sums + p.parts + batch * (3 * p.x + 5 * p.mm);
     return p;
 }
@@ -920,7 +939,8 @@ void gemm(Gemm a, int M, int N, bool turn, int batch, int dtype, const Ptrs &p, 
 {
     a.batch = batch;
     if (a.D2) batch *= 2;
-    // 128 x 128 tiles halve the operand traffic of 64 x 64 ones, but a launch should have a workgroup for every CU
+    // 128 x 128 tiles halve the operand traffic of 64 x 64 ones, but most CUs should have one (2304 x 2304, 171 symmetric tiles:
+    // 53 us either way; 210 of them 60 against 82 us)
     const auto tiles = [&](int t) { return a.symmetric ? (long long)(M / t) * (M / t + 1) / 2 : (long long)(M / t) * (N / t); };
     const bool big = M % 128 == 0 && N % 128 == 0 && tiles(128) * batch >= BIG_TILES;
     const int t = big ? 128 : 64;
@@ -929,32 +949,54 @@ void gemm(Gemm a, int M, int N, bool turn, int batch, int dtype, const Ptrs &p, 
     a.tiles_m = M / t;
     a.tiles_n = N / t;
     // workgroups that leave CUs with one or two of them get more wavefronts each
-    const int ks = big ? 1 : groups <= FEW_TILES ? 4 : groups <= 2 * FEW_TILES ? 2 : 1;
-    // Gram matrices of few tiles and a long K: a round of a workgroup (KS stages) takes about 1 us, joining the shares of
-    // several workgroups 4.5 us
+    int ks = big ? (groups <= CUS ? 2 : 1) : groups <= FEW_TILES ? 4 : groups <= 2 * FEW_TILES ? 2 : 1;
     a.split = 1;
+    long long whole = groups;
     if (turn && ks == 4) {
+        // Gram matrices of few tiles and a long K: a round of a workgroup (KS stages) takes about 1 us, joining the shares
+        // of several workgroups 4.5 us
         const int rounds = (a.K / BK + 3) / 4;
         int most = (int)(FEW_TILES / groups);
         if (most > (rounds + 1) / 2) most = (rounds + 1) / 2;
-        if (most > 1 && rounds - (rounds + most - 1) / most >= 6) a.split = most;
-        if (a.poly) a.split = most;
+        if (a.poly || (most > 1 && rounds - (rounds + most - 1) / most >= 6)) {
+            a.split = most;
+            whole = 0;
+        }
+    } else if (big && groups > CUS && groups < 4 * CUS && a.K >= 2048) {
+        // A few large tiles more than CUs: a CU that gets another one doubles its time, so the last ones are shared by as
+        // many workgroups as there are CUs.  272 tiles, K = 4096 / 2048: 151 / 85 us -> 116 + 9 / 67 + 10 us (with the
+        // joining); 288 tiles, K = 1024: 46 -> 43 + 7 us, so not there.
+        const long long rest = groups % CUS;
+        if (rest && rest <= CUS / 2) {
+            ks = 2;
+            a.split = (int)(CUS / rest);
+            if (a.split > a.K / BK / 4) a.split = a.K / BK / 4;
+            whole = groups - rest;
+        }
     }
-    if (a.split == 1 && !a.poly) a.parts = nullptr;
-    const dim3 grid((unsigned)(groups * a.split)), block(256 * ks);
+    a.whole = (int)whole;
+    const long long shared = groups - whole;
+    const dim3 grid((unsigned)(whole + shared * a.split)), block(256 * ks);
     const auto go = [&](auto *kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, a, p, s); };
     const auto run = [&](auto turn, auto *d) {
         using T = std::remove_pointer_t<decltype(d)>;
         constexpr bool TURN = decltype(turn)::value;
-        if (big) go(k_gemm<128, 128, 1, TURN, T>);
-        else if (ks == 4) go(k_gemm<64, 64, 4, TURN, T>);
+        if constexpr (!TURN) { // (Gram matrices of large tiles are computed from X by rows)
+            if (big) {
+                if (ks == 2) go(k_gemm<128, 128, 2, false, T>);
+                else go(k_gemm<128, 128, 1, false, T>);
+                if (shared) hipLaunchKernelGGL((k_join<128, T>), dim3((unsigned)shared * 4), dim3(256), 0, st, a, p, s);
+                return;
+            }
+        }
+        if (ks == 4) go(k_gemm<64, 64, 4, TURN, T>);
         else if (ks == 2) go(k_gemm<64, 64, 2, TURN, T>);
         else go(k_gemm<64, 64, 1, TURN, T>);
     };
     if (turn) {
         run(std::true_type(), (float *)nullptr);
         if (a.poly) hipLaunchKernelGGL(k_join_poly, dim3((unsigned)groups), dim3(256), 0, st, a);
-        else if (a.parts) hipLaunchKernelGGL(k_join, dim3((unsigned)groups), dim3(256), 0, st, a, p, s);
+        else if (shared) hipLaunchKernelGGL((k_join<64, float>), dim3((unsigned)groups), dim3(256), 0, st, a, p, s);
     }
     else if (a.D) run(std::false_type(), (float *)nullptr);
     else by_type(dtype, [&](auto *d) { run(std::false_type(), d); });
@@ -1026,6 +1068,7 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
         g.E = E; g.beta = beta; g.gamma = gamma;
         g.D = out;
         g.A2 = x2; g.B2 = y2; g.D2 = out2;
+        g.parts = parts_at;
         gemm(g, s.mp, s.mp, false, batch, dtype, p, s, st);
     };
     // Steps per group.  float32 results take every step on X (the error stays at or below that of float32 products).
@@ -1082,6 +1125,7 @@ int run_batch(int batch, Shape s, int dtype, int steps, const Ptrs &p, char *wor
         g.pitchA = g.pitchB = pm;
         g.K = s.mp;
         g.alpha = two((left ? EXP_X : 0) - EXP_Q - EXP_X);
+        g.parts = parts_at;
         if (left) {
             g.sD = pl.x;
             g.D = YT;

@@ -72,6 +72,27 @@ def test_numbers_of_steps(steps, shape):
         assert 0.6 < s.min() and s.max() < 1.25
 
 
+@pytest.mark.parametrize("shape,dtype", [((2, 2048, 2100), torch.float32), ((1, 2050, 2300), torch.float32), ((2300, 2100), torch.bfloat16),
+                                         ((1, 2600, 2500), torch.float16)])
+def test_large_tiles_that_workgroups_share(shape, dtype):
+    # a few tiles more than there are CUs (symmetric, two products at once, the last product in each type), and a few less
+    from alphazero_amd import muon
+
+    g = _updates(shape, 17).to(dtype).cuda()
+    out = muon.orthogonalise(g, 4)
+    assert torch.equal(out, muon.orthogonalise(g, 4))
+    x = g.double()  # (the definition on the GPU, in 64 bits)
+    x = x.transpose(-1, -2).contiguous() if x.shape[-2] > x.shape[-1] else x
+    x = x / x.square().sum((-1, -2), keepdim=True).sqrt()
+    for _ in range(4):
+        A = x @ x.transpose(-1, -2).contiguous()
+        x = ABC[0] * x + (ABC[1] * A + ABC[2] * (A @ A)) @ x
+    x = x.transpose(-1, -2) if shape[-2] > shape[-1] else x
+    off, size = (out.double() - x).flatten(-2).norm(dim=-1), x.flatten(-2).norm(dim=-1)
+    tol = ABC[0] ** 3 * 1.41 * 32 * U + size * (64 * U + (torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0))
+    assert (off <= tol).all(), (off, tol)
+
+
 @pytest.mark.parametrize("shape", [(3, 64, 2304), (4608, 20), (300, 4000), (2, 129, 3000), (300, 33, 800), (2, 1500, 40), (1, 1050, 1400)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_long_gram_sums_and_large_tiles(shape, dtype):
