@@ -906,7 +906,8 @@ template <class F> void by_type(int dtype, F f)
 
 int round_up(int v, int to) { return (v + to - 1) / to * to; }
 
-Shape shape_of(int rows, int cols)
+// (count: matrices of the call)
+Shape shape_of(int rows, int cols, int count)
 {
     Shape s = {};
     s.rows = rows;
@@ -914,8 +915,11 @@ Shape shape_of(int rows, int cols)
     s.tall = rows > cols;
     s.m = s.tall ? cols : rows;
     s.n = s.tall ? rows : cols;
-    s.mp = round_up(s.m, s.m <= 64 ? 64 : 128);
-    s.np = round_up(s.n, s.n <= 64 ? 64 : 128);
+    // to whole large tiles only where the product X <- Q X has enough of them (20 x 150 x 300 padded to 128: 131 us, to 64: 115;
+    // 4 x 400 x 1100 198 and 180 us)
+    const bool big = s.m > 64 && (long long)((s.m + 127) / 128) * ((s.n + 127) / 128) * (count < MAX_BATCH ? count : MAX_BATCH) >= BIG_TILES;
+    s.mp = round_up(s.m, big ? 128 : 64);
+    s.np = round_up(s.n, big ? 128 : 64);
     return s;
 }
 
@@ -1168,7 +1172,7 @@ long long az_muon_work(int count, int rows, int cols)
 {
     if (!shape_ok(count, rows, cols, AZ_F32, 1)) return -1;
     if (count == 0) return 0;
-    const Shape s = shape_of(rows, cols);
+    const Shape s = shape_of(rows, cols, count);
     return is_small(s) ? 0 : (long long)plan_of(s, batch_of(s, count)).total;
 }
 
@@ -1180,7 +1184,7 @@ int az_muon_orthogonalise(int count, int rows, int cols, const void *const *d_in
     if (!d_in || !d_out) return AZ_ERR_ARG;
     for (int i = 0; i < count; i++)
         if (!d_in[i] || !d_out[i]) return AZ_ERR_ARG;
-    Shape s = shape_of(rows, cols);
+    Shape s = shape_of(rows, cols, count);
     s.ld_in = ld_in;
     s.ld_out = ld_out;
     const bool small = is_small(s);
