@@ -204,6 +204,27 @@ __device__ __forceinline__ h8 turned(const char *a, const char *b)
     return u.h;
 }
 
+// Four of those at LDS addresses (bytes) + AT, their second halves FURTHER bytes behind.  The builtin is taken for a read of
+// what any load into LDS may still write: the compiler waits for all of them before it, also for the stage that was just
+// asked for.  These reads are waited for within the block.
+template <int AT, int FURTHER> __device__ __forceinline__ void turned4(unsigned a, unsigned b, unsigned c, unsigned d, h8 &ra, h8 &rb, h8 &rc, h8 &rd)
+{
+    union { struct { s4 a, b; } s; h8 h; } u, v, w, x;
+    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %2, %9 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %4, %10 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %6, %11 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(u.s.a), "=&v"(u.s.b), "=&v"(v.s.a), "=&v"(v.s.b), "=&v"(w.s.a), "=&v"(w.s.b), "=&v"(x.s.a), "=&v"(x.s.b)
+                 : "v"(a), "v"(b), "v"(c), "v"(d), "n"(AT), "n"(AT + FURTHER)
+                 : "memory");
+    ra = u.h; rb = v.h; rc = w.h; rd = x.h;
+}
+
 constexpr int BK = 32;              // K per stage: 128 bytes of a packed row
 // place of 16-byte piece c of row r within the row's 128 bytes: 16 lanes that read the same piece of 16 rows touch
 // all 64 banks
@@ -309,25 +330,25 @@ __device__ __forceinline__ void store_tile(float *t, const Gemm &a, const Ptrs &
 }
 
 // BM x BN results per workgroup of 4 wavefronts (2 x 2); per stage and wavefront (BM/64) (BN/64) 2 x 3 matrix
-// instructions 32x32x16 on (BM/64 + BN/64) 4 LDS reads.  Two stages in LDS: the next one loads while this one is used.
+// instructions 32x32x16 on (BM/64 + BN/64) 4 LDS reads.  D places for stages in LDS: D - 1 load while one is used.
 // KS groups of 4 wavefronts take every KS-th stage of K, each with stages of its own, and add up at the end: where tiles
-// are few a CU needs more loads in flight (what one asks for arrives after 2100 cycles).  Measured with one group /
-// four: 256 x 2304, one matrix 225 / 174 us, 4 x 512 x 512 191 / 153 us.  (Every wavefront on its own, a whole tile each,
-// with four pieces of K in flight: 200 and 173 us.)  Large tiles: a CU that has one workgroup of two groups is busy, with
-// one of one group it waits (210 symmetric tiles, K = 2560: 60 us; as 820 tiles of 64, four to a CU: 82 us).
+// are few a CU needs more loads in flight (what one asks for arrives after 2100 cycles).  Measured with one group and two
+// places / several: 256 x 2304, one matrix 225 / 137 us, 4 x 512 x 512 191 / 151 us.  (Every wavefront on its own, a whole
+// tile each, with four pieces of K in flight, took 200 us where four groups took 174.)  Large tiles: a CU that has one workgroup of two
+// groups is busy, with one of one group it waits (210 symmetric tiles, K = 2560: 60 us; as 820 tiles of 64, four to a CU: 82 us).
 // The last tiles may be shared: workgroups take parts of their K and leave float32 sums for k_join.
 // TURN: A and B are given as [K][M] and [K][N] (the Gram matrix from X'), and the LDS reads transpose.
-template <int BM, int BN, int KS, bool TURN, class T>
+template <int BM, int BN, int KS, int D, bool TURN, class T>
 __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs p, Shape s)
 {
     constexpr int FM = BM / 64, FN = BN / 64; // 32 x 32 blocks of a wavefront
     constexpr int STAGE = (BM + BN) * 128;
     constexpr int TILE = BN * (BM + 4) * 4;
-    __shared__ __align__(16) char lds_all[KS * (2 * STAGE > TILE ? 2 * STAGE : TILE)];
+    __shared__ __align__(16) char lds_all[KS * (D * STAGE > TILE ? D * STAGE : TILE)];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
     const int group = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
-    char *lds = lds_all + group * 2 * STAGE;
-    constexpr bool SHARES = BM == 64 ? TURN && KS == 4 : KS == 2; // some tiles may be shared
+    char *lds = lds_all + group * D * STAGE;
+    constexpr bool SHARES = BM == 64 ? TURN && D == 4 : KS == 2; // some tiles may be shared
     // workgroups go round the 8 XCDs: each XCD gets a run of neighbouring tiles, which share operands in its L2
     int item, share = -1, b, ti, tj;
     {
@@ -404,34 +425,40 @@ __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs
 #pragma unroll
         for (int l = 0; l < LOADS; l++) src[l] += (size_t)first * (l * 4 < BM / 8 ? next_a : next_b);
     }
-    if (group < stages) load_stage(group, lds);
-    const int rounds = (stages + KS - 1) / KS;
-    for (int k = 0; k < rounds; k++) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // this wavefront's part of stage k has arrived
-        __syncthreads();                                 // all of it has; nobody reads the other buffer any more
-        const char *cur = lds + (k & 1) * STAGE;
-        const int after = (k + 1) * KS + group;
-        if (after < stages) load_stage(after, lds + ((k + 1) & 1) * STAGE);
-        if (KS > 1 && k * KS + group >= stages) break; // (the last round; this group's share is done)
 #pragma unroll
-        for (int ks = 0; ks < 2; ks++) {
+    for (int d = 0; d < D - 1; d++) {
+        if (d * KS + group < stages) load_stage(d * KS + group, lds + d * STAGE);
+        asm volatile("" ::: "memory"); // (in this order: the waits below count loads)
+    }
+    // (one way out of the loop: where there were two the compiler counted the wait states between the last products and the
+    // first use of their results along the longer one, and results came without the last products)
+    const int rounds = (stages + KS - 1) / KS, mine = KS == 1 ? rounds : (stages - group + KS - 1) / KS; // of all groups, of this one
+    int at = 0, to = D - 1; // places of this round's stage and of the one that is asked for
+    for (int k = 0; k < mine; k++) {
+        // this wavefront's part of the group's stage k has arrived (loads arrive in order, up to D - 2 stages of them stay
+        // behind it), and it has read all it wanted of stage k - 1
+        static_assert(D == 2 || D == 4, "the waits below");
+        const int next = (k + 1) * KS + group;
+        if (D == 4 && next + KS < stages) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * LOADS) : "memory");
+        else if (D == 4 && next < stages) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier(); // (not __syncthreads(), which would wait for all loads)
+        asm volatile("" ::: "memory");
+        const char *cur = lds + at * STAGE;
+        const int after = (k + D - 1) * KS + group;
+        if (after < stages) load_stage(after, lds + to * STAGE);
+        at = at + 1 == D ? 0 : at + 1;
+        to = to + 1 == D ? 0 : to + 1;
+        const auto half_stage = [&](auto which) {
+            constexpr int ks = decltype(which)::value;
             h8 ah[FM], al[FM], bh[FN], bl[FN];
-            if (TURN) {
-                const int q = lane & 3, kk = ks * 16 + half * 8 + (lane >> 2 & 3), f = place_k(kk, 0), up = (lane >> 4 & 1) * 4 + (q & 2);
-#pragma unroll
-                for (int i = 0; i < FM; i++) {
-                    const char *at = cur + kk * BM * 4 + (q & 1) * 8;
-                    const int c = (wm + i * 32) / 4 + up;
-                    ah[i] = turned(at + (c ^ f) * 16, at + 4 * BM * 4 + (c ^ f) * 16);
-                    al[i] = turned(at + ((c + 1) ^ f) * 16, at + 4 * BM * 4 + ((c + 1) ^ f) * 16);
-                }
-#pragma unroll
-                for (int j = 0; j < FN; j++) {
-                    const char *at = cur + BM * 128 + kk * BN * 4 + (q & 1) * 8;
-                    const int c = (wn + j * 32) / 4 + up;
-                    bh[j] = turned(at + (c ^ f) * 16, at + 4 * BN * 4 + (c ^ f) * 16);
-                    bl[j] = turned(at + ((c + 1) ^ f) * 16, at + 4 * BN * 4 + ((c + 1) ^ f) * 16);
-                }
+            if constexpr (TURN) {
+                static_assert(!TURN || (FM == 1 && FN == 1 && BM == BN), "one block of each operand");
+                const int q = lane & 3, kk = half * 8 + (lane >> 2 & 3), f = place_k(kk, 0), up = (lane >> 4 & 1) * 4 + (q & 2);
+                const unsigned at = (unsigned)(size_t)(const __attribute__((address_space(3))) char *)cur + kk * BM * 4 + (q & 1) * 8;
+                const int ca = wm / 4 + up, cb = wn / 4 + up;
+                turned4<ks * 16 * BM * 4, 4 * BM * 4>(at + (ca ^ f) * 16, at + ((ca + 1) ^ f) * 16, at + BM * 128 + (cb ^ f) * 16,
+                                                      at + BM * 128 + ((cb + 1) ^ f) * 16, ah[0], al[0], bh[0], bl[0]);
             } else {
                 const int c = (ks * 2 + half) * 2;
 #pragma unroll
@@ -457,8 +484,11 @@ __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs
                     }
                     acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
                 }
-        }
+        };
+        half_stage(std::integral_constant<int, 0>());
+        half_stage(std::integral_constant<int, 1>());
     }
+    if (mine < rounds) __builtin_amdgcn_s_barrier(); // (the last round has no stage for this group)
     __syncthreads();
     float *t = (float *)lds_all, *part = (float *)(lds_all + group * TILE);
 #pragma unroll
@@ -957,8 +987,8 @@ void gemm(Gemm a, int M, int N, bool turn, int batch, int dtype, const Ptrs &p, 
     a.split = 1;
     long long whole = groups;
     if (turn && ks == 4) {
-        // Gram matrices of few tiles and a long K: a round of a workgroup (KS stages) takes about 1 us, joining the shares
-        // of several workgroups 4.5 us
+        // Gram matrices of few tiles and a long K: four stages of a workgroup take about 0.8 us, joining the shares of
+        // several workgroups 4.5 us
         const int rounds = (a.K / BK + 3) / 4;
         int most = (int)(FEW_TILES / groups);
         if (most > (rounds + 1) / 2) most = (rounds + 1) / 2;
@@ -980,6 +1010,11 @@ void gemm(Gemm a, int M, int N, bool turn, int batch, int dtype, const Ptrs &p, 
     }
     a.whole = (int)whole;
     const long long shared = groups - whole;
+    // Two groups with four places each ask for six stages at once.  That matters more than wavefronts for Gram matrices (1 x
+    // 1024 x 1024 199 -> 196 us in all) and up to 12 stages (64 x 100 x 200 207 -> 196 us); other products of 40 stages are
+    // faster with four groups (5 x 1201 x 333 193, 206 us).
+    const bool deep = ks == 4 && (turn || a.K / BK / a.split <= 12);
+    if (deep) ks = 2;
     const dim3 grid((unsigned)(whole + shared * a.split)), block(256 * ks);
     const auto go = [&](auto *kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, a, p, s); };
     const auto run = [&](auto turn, auto *d) {
@@ -987,15 +1022,18 @@ void gemm(Gemm a, int M, int N, bool turn, int batch, int dtype, const Ptrs &p, 
         constexpr bool TURN = decltype(turn)::value;
         if constexpr (!TURN) { // (Gram matrices of large tiles are computed from X by rows)
             if (big) {
-                if (ks == 2) go(k_gemm<128, 128, 2, false, T>);
-                else go(k_gemm<128, 128, 1, false, T>);
+                if (ks == 2) go(k_gemm<128, 128, 2, 2, false, T>);
+                else go(k_gemm<128, 128, 1, 2, false, T>);
                 if (shared) hipLaunchKernelGGL((k_join<128, T>), dim3((unsigned)shared * 4), dim3(256), 0, st, a, p, s);
                 return;
             }
         }
-        if (ks == 4) go(k_gemm<64, 64, 4, TURN, T>);
-        else if (ks == 2) go(k_gemm<64, 64, 2, TURN, T>);
-        else go(k_gemm<64, 64, 1, TURN, T>);
+        if constexpr (!TURN) {
+            if (ks == 4) return go(k_gemm<64, 64, 4, 2, false, T>);
+        }
+        if (deep) go(k_gemm<64, 64, 2, 4, TURN, T>);
+        else if (ks == 2) go(k_gemm<64, 64, 2, 2, TURN, T>);
+        else go(k_gemm<64, 64, 1, 2, TURN, T>);
     };
     if (turn) {
         run(std::true_type(), (float *)nullptr);

@@ -133,7 +133,10 @@ def test_low_rank_sizes_and_zeros(shape):
             assert shape[0] < 3 or torch.isfinite(got[2]).all()
 
 
-@pytest.mark.parametrize("shape", [(8, 16, 144), (8, 30, 600), (8, 64, 576), (2, 64, 4000), (2, 128, 1024), (1, 500, 2048)])
+@pytest.mark.parametrize("shape", [(8, 16, 144), (8, 30, 600), (8, 64, 576), (2, 64, 4000), (2, 128, 1024), (1, 500, 2048),
+                                   # whole tiles and stages, so that no padding hides a missing product: few and many workgroups
+                                   (32, 192, 768), (300, 64, 1024), (3, 128, 256), (200, 128, 512), (5, 256, 1056), (1, 512, 2048),
+                                   (1, 128, 8192), (8, 512, 1024), (2, 1024, 4096), (6, 384, 1536)])
 def test_every_number_of_wide_matrices_has_float32_precision(shape):
     # The singular values of a wide random matrix lie close together, so no direction's error outgrows the others: five
     # steps of at most 8 u each (the bound above) and as much again for their mutual growth are 80 u.  One number of X or Q
