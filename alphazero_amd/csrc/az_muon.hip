@@ -974,7 +974,8 @@ Plan plan_of(const Shape &s, int batch)
     p.x = (size_t)s.mp * s.np * 4;
     p.mm = (size_t)s.mp * s.mp * 4;
     p.sums = (size_t)batch * NORM_PARTS * sizeof(double);
-    p.parts = (size_t)CUS * 128 * 128 * 4; // sums of shared tiles: at most a large one for every CU
+    const size_t side = s.mp % 128 == 0 ? 128 : 64;
+    p.parts = CUS * side * side * 4; // sums of shared tiles: at most one for every CU
     p.total = p.sums + p.parts + batch * (3 * p.x + 5 * p.mm);
     return p;
 }
@@ -1199,7 +1200,8 @@ int batch_of(const Shape &s, int count)
 {
     long long most = MAX_BATCH;
     if (!is_small(s)) {
-        const long long fit = (long long)(((size_t)1 << 30) / plan_of(s, 1).total);
+        const Plan one = plan_of(s, 1);
+        const long long fit = (long long)((((size_t)1 << 30) - one.parts) / (one.total - one.parts));
         most = fit < 1 ? 1 : fit < most ? fit : most;
     }
     return (int)(count < most ? count : most);

@@ -62,3 +62,12 @@ def test_optimiser_refuses_later_groups():
         assert len(opt.param_groups) == 1
     opt.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(2, 5))], lr=0.1))
     assert len(opt.param_groups) == 2
+
+
+def test_workspace_grows_with_the_batch_and_ends():
+    L = E.load_library()
+    one, many = L.az_muon_work(1, 100, 400), L.az_muon_work(200, 100, 400)
+    assert one < 18 << 20 and many > 200 * 3 * 100 * 400 * 4  # (16 MiB of sums of shared tiles) one launch for all
+    for shape in ((100, 400), (1000, 1000), (70, 20000)):
+        assert L.az_muon_work(100000, *shape) <= (1 << 30) + 4096
+    assert L.az_muon_work(3, 16384, 16384) > 0
