@@ -404,11 +404,10 @@ __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs
 #pragma unroll
         for (int l = 0; l < LOADS; l++) load_lds(src[l] + (size_t)k * (l * 4 < BM / 8 ? next_a : next_b), to + dst[l]);
     };
-    // A result of bfloat16 is rounded at 2^-9: its last product needs no small products (they are below 2^-11, and nothing
-    // multiplies that error any more).
-    constexpr bool LOW = !std::is_same<T, bf16_t>::value;
-    // the small products have accumulators of their own: added to the large ones they would cost a rounding each
-    // (three times the error of one step)
+    // The small products have accumulators of their own: added to the large ones they would cost a rounding each
+    // (three times the error of one step).  They stay in the last product of a bfloat16 result too: without them its error is
+    // 2^-12 of |Q| |X|, and Q is a^k = 41 (three steps) where X has next to nothing, four times the type's rounding on an
+    // update of low rank.
     f16v acc[FM][FN], low[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; i++)
@@ -478,10 +477,8 @@ __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs
             for (int i = 0; i < FM; i++)
 #pragma unroll
                 for (int j = 0; j < FN; j++) {
-                    if (LOW) {
-                        low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], low[i][j], 0, 0, 0);
-                        low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], low[i][j], 0, 0, 0);
-                    }
+                    low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], low[i][j], 0, 0, 0);
+                    low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], low[i][j], 0, 0, 0);
                     acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
                 }
         };
@@ -499,7 +496,7 @@ __global__ __launch_bounds__(256 * KS, KS < 3 ? 2 : KS) void k_gemm(Gemm a, Ptrs
             for (int e = 0; e < 16; e += 4) {
                 float v[4];
 #pragma unroll
-                for (int q = 0; q < 4; q++) v[q] = (LOW ? acc[i][j][e + q] + low[i][j][e + q] : acc[i][j][e + q]) * a.alpha;
+                for (int q = 0; q < 4; q++) v[q] = (acc[i][j][e + q] + low[i][j][e + q]) * a.alpha;
                 *(float4 *)(part + tile_place<BM>(wm + i * 32 + e * 2 + half * 4, wn + j * 32 + lr)) = make_float4(v[0], v[1], v[2], v[3]);
             }
     __syncthreads();

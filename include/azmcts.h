@@ -483,9 +483,10 @@ int az_policy_loss(int n, int actions, const void *d_logits, int dtype, long lon
  * AZ_BF16 / AZ_F16): X = G / |G|_F, then `steps` times X <- a X + (b A + c A^2) X with A = X X' (X' X for a matrix taller
  * than wide) and (a, b, c) = (3.4445, -4.7750, 2.0315), to d_out[i] [rows][ld_out] in the same type (d_out[i] may be
  * d_in[i]; outputs overlap nothing else).  A matrix of zeros stays zero, one with an infinity or NaN becomes NaN.  The
- * products have float32 precision (the last of a bfloat16 result that of its rounding); the same call gives the same
- * bits (how many matrices there are decides how sums are split, so a matrix alone may differ in the last bits).  d_work: az_muon_work(count, rows, cols) bytes (0 for small matrices), used by this call only; the device current
- * at the call is the one of the pointers and of `stream`. */
+ * products have float32 precision whatever the type, and a result is rounded to its type once; the same call gives the same
+ * bits (how many matrices there are decides how sums are split, so a matrix alone may differ in the last bits).  d_work:
+ * az_muon_work(count, rows, cols) bytes (0 for small matrices), used by this call only; the device current at the call is
+ * the one of the pointers and of `stream`. */
 enum { AZ_MUON_MAX_DIM = 32768, AZ_MUON_MAX_CELLS = 1 << 28, AZ_MUON_MAX_STEPS = 20 };
 long long az_muon_work(int count, int rows, int cols);
 int az_muon_orthogonalise(int count, int rows, int cols, const void *const *d_in, long long ld_in, void *const *d_out,

@@ -326,3 +326,23 @@ def test_records_to_update_together():
         u = _exact((1.95 * p.grad).flatten(1).cpu()).view(p.shape)  # first step: m = g, u = g + 0.95 g
         want = b.cpu().double() - 0.02 * max(1.0, p.shape[0] / p[0].numel()) ** 0.5 * u
         assert (p.detach().cpu().double() - want).norm() < 1e-5 * want.norm()
+
+
+# widths from 1.5 times the height on, more than 64 rows: tiles of 64 (Gram matrices shared and not) and of 128
+@pytest.mark.parametrize("shape", [(256, 2304), (512, 1024), (70, 130), (333, 1201), (1500, 130), (12, 256, 768)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rank,floor", [(1, None), (4, None), (1, 0.0), (4, 0.0), (32, 0.0), (64, 0.02)])
+def test_low_rank_updates_in_16_bits(shape, dtype, rank, floor):
+    # Gradients of a batch smaller than the layer: most directions hold nothing, or only noise, and every step multiplies
+    # what a rounded product leaves in them by a.  Same bound as above: products of float32 precision, one rounding.
+    from alphazero_amd import muon
+
+    g = _updates(shape, 31, 1.0, rank=rank)
+    if floor is None:  # small whole numbers: exactly of that rank in every type
+        gen = torch.Generator().manual_seed(33)
+        g = (torch.randint(-2, 3, (*shape[:-1], rank), generator=gen) @ torch.randint(-2, 3, (*shape[:-2], rank, shape[-1]), generator=gen)).float()
+    elif floor:
+        g = g + floor * math.sqrt(rank) * _updates(shape, 32, 1.0)
+    g = g.to(dtype).cuda()
+    for steps in (3, 4, 5, 6, 7):
+        _check(muon.orthogonalise(g, steps), g, steps)
