@@ -122,7 +122,8 @@ __device__ __forceinline__ float as_float(f16_t v) { return (float)v.h; }
 
 // The row's cells of this lane, -inf where the mask or the row's end leaves nothing (a select: what stands in a masked
 // place is never computed with).  The logits are asked for before the mask, so that the row waits for memory once.
-template <class T, int R> __device__ __forceinline__ void load_row(const Rows &a, size_t row, int lane, float (&x)[R])
+// q: numbers that go with the cells, 0 in those places (a legal cell may hold -inf too, and keeps its number).
+template <class T, int R> __device__ __forceinline__ void load_row(const Rows &a, size_t row, int lane, float (&x)[R], float *q = nullptr)
 {
     const T *p = (const T *)a.x + row * (size_t)a.ld;
     T raw[R];
@@ -152,7 +153,11 @@ template <class T, int R> __device__ __forceinline__ void load_row(const Rows &a
         for (int r = 0; r < R; r++) ok[r] = true;
     }
 #pragma unroll
-    for (int r = 0; r < R; r++) x[r] = ok[r] && r * 64 + lane < a.A ? as_float(raw[r]) : NINF;
+    for (int r = 0; r < R; r++) {
+        const bool in = ok[r] && r * 64 + lane < a.A;
+        x[r] = in ? as_float(raw[r]) : NINF;
+        if (q) q[r] = in ? q[r] : 0.f;
+    }
 }
 
 struct Stats { float M, logS, H; bool live; };
@@ -419,6 +424,16 @@ struct Loss {
 // log pi, finite for 0 (which multiplies it); NaN for a negative one
 __device__ __forceinline__ float log_of(float pi) { return pi == 0.f ? 0.f : __logf(pi); }
 
+// pi (log pi - d) for d = x - M: 0 without a target, +inf for a target where the difference is -inf
+__device__ __forceinline__ float miss_of(float pi, float d) { return pi * (pi == 0.f ? 0.f : __logf(pi) - d); }
+
+// the gradient of a cell, e = e^(x - M) and inv = sum pi / S: 0 where the mask leaves nothing, -pi for a target at -inf
+__device__ __forceinline__ float slope_of(float x, float e, float inv, float pi, float f)
+{
+    const float g = (x == NINF ? 0.f : e * inv) - pi;
+    return x == NINF && pi == 0.f ? 0.f : g * f;
+}
+
 // sums of a workgroup's wavefronts in wavefront order
 template <int W> __device__ __forceinline__ void block_part(double p, double v, double *out)
 {
@@ -470,7 +485,7 @@ template <class T, int R> __global__ __launch_bounds__(64 * WAVES) void k_loss(R
         float x[R], q[R];
 #pragma unroll
         for (int r = 0; r < R; r++) q[r] = pi[min(r * 64 + lane, a.A - 1)];
-        load_row<T, R>(a, row, lane, x);
+        load_row<T, R>(a, row, lane, x, q); // (masked places and cells past the row's end hold no target)
         float m = x[0];
 #pragma unroll
         for (int r = 1; r < R; r++) m = fmaxf(m, x[r]);
@@ -479,12 +494,11 @@ template <class T, int R> __global__ __launch_bounds__(64 * WAVES) void k_loss(R
         float s = 0.f, w = 0.f, l = 0.f, e[R];
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            q[r] = x[r] == NINF ? 0.f : q[r]; // masked places (and cells past the row's end) hold no target
-            float d;
-            e[r] = term(x[r], M, d);
+            const float d = x[r] - M;
+            e[r] = exp_neg(d);
             s += e[r];
             w += q[r];
-            l += q[r] * (log_of(q[r]) - d);
+            l += miss_of(q[r], d);
         }
         s = wave_sum(s);
         w = wave_sum(w);
@@ -499,7 +513,7 @@ template <class T, int R> __global__ __launch_bounds__(64 * WAVES) void k_loss(R
             T *out = (T *)o.dx + (size_t)row * a.A;
 #pragma unroll
             for (int r = 0; r < R; r++)
-                if (r * 64 + lane < a.A) put(out, r * 64 + lane, x[r] == NINF ? 0.f : (e[r] * inv - q[r]) * f);
+                if (r * 64 + lane < a.A) put(out, r * 64 + lane, slope_of(x[r], e[r], inv, q[r], f));
         }
     }
     const double v = value_part<T>(a, o, scale);
@@ -584,7 +598,8 @@ template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_parts(Ro
         float m = NINF;
 #pragma unroll
         for (int r = 0; r < LONG_R; r++) {
-            x[r] = ok[r] && j0 + r * 64 + lane < end ? x[r] : NINF;
+            ok[r] = ok[r] && j0 + r * 64 + lane < end;
+            x[r] = ok[r] ? x[r] : NINF;
             m = fmaxf(m, x[r]);
         }
         m = wave_max(m);
@@ -602,10 +617,10 @@ template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_parts(Ro
             S += e;
             U += e == 0.f ? 0.f : e * d;
             if (pi) {
-                const float w = x[r] == NINF ? 0.f : q[r];
+                const float w = ok[r] ? q[r] : 0.f;
                 W += w;
                 E += w * log_of(w);
-                X += w == 0.f ? 0.f : w * d;
+                X += w == 0.f ? 0.f : w * (x[r] == NINF ? NINF : d); // (M is -inf until a cell above it comes)
             }
         }
         if (o.top) best_offer<LONG_R>(best, x, j0, o.top, lane);
@@ -812,8 +827,8 @@ template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_loss(Row
         const int begin = chunk * c.len, end = min(a.A, begin + c.len);
         const Part t = join_parts(part + (size_t)row * c.count, c.count, lane);
         const bool live = t.S != 0.f;
-        if (chunk == 0 && lane == 0 && live) {
-            const float logS = logf(t.S);
+        if (chunk == 0 && lane == 0) {
+            const float logS = live ? logf(t.S) : 0.f;
             sum += (double)t.E - (double)t.X + (double)logS * (double)t.W;
         }
         if (!o.dx) continue;
@@ -834,7 +849,7 @@ template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_loss(Row
 #pragma unroll
             for (int r = 0; r < LONG_R; r++)
                 if (j0 + r * 64 + lane < end)
-                    put(out, j0 + r * 64 + lane, !ok[r] || x[r] == NINF ? 0.f : (exp_neg(x[r] - t.M) * inv - q[r]) * f);
+                    put(out, j0 + r * 64 + lane, ok[r] ? slope_of(x[r], exp_neg(x[r] - t.M), inv, q[r], f) : 0.f);
         }
     }
     const double v = value_part<T>(a, o, scale);

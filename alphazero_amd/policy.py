@@ -245,7 +245,8 @@ def loss(logits, value, pi, r, *, board=None, legal=None, parts=False):
 
     logits  [n, actions] float32, bfloat16 or float16, p their softmax over the legal moves (see `score` for board and
             legal; the reference trains without a mask);  value  n values of any shape, float32 or the logits' type
-    pi      float32 [n, actions], targets (rows need not sum to 1; masked cells are not looked at);  r  float32, n results
+    pi      float32 [n, actions], targets (rows need not sum to 1; masked cells are not looked at, a target on a legal cell
+            at -inf makes the loss infinite);  r  float32, n results
 
     Differentiable (once) for logits and value.  parts=True returns (total, policy part, value part), the parts without
     gradient.  Zero records give 0."""

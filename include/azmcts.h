@@ -465,7 +465,9 @@ int az_policy_score_grad(int n, int actions, const void *d_logits, int dtype, lo
                          const void *d_moves, int move_bytes, int m, const float *d_g_logp, const float *d_g_entropy,
                          const float *d_entropy, const float *d_stats, void *d_dlogits, void *stream);
 /* The trainer's loss over n >= 1 records:  1/n sum_i sum_j pi_ij (log pi_ij - log p_ij) + 1/n sum_i (v_i - r_i)^2,
- * j over the legal cells (targets in masked cells are not looked at, 0 log 0 = 0, an empty row adds its value part only).
+ * j over the legal cells (targets in masked cells are not looked at, 0 log 0 = 0, a row without a legal cell adds its
+ * value part only).  A legal cell at -inf has log p = -inf, so a target there makes the loss +inf (and its gradient
+ * -pi / n); the same holds where x_j lies further below the row's maximum than float32 can say.
  *   d_value [n]: float32 (value_f32) or the logits' type; d_pi float32 [n][actions]; d_r float32 [n]
  *   d_loss [1] (may be NULL): the total; d_parts [2] (may be NULL): policy part, value part
  *   d_dlogits [n][actions] (type of the logits), d_dvalue [n] (type of the values): gradients of the total times

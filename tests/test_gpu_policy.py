@@ -445,3 +445,69 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for k, s in enumerate(got):
         assert all(torch.equal(a, b) for a, b in zip(s, want[k % 2])), k
+
+
+@pytest.mark.parametrize("actions", [5, 225, 1024, 1500, 70000])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_loss_where_a_legal_move_has_no_probability(actions, dtype):
+    # A legal cell at -inf has log-probability -inf: a target there makes the loss infinite (as torch's own kl_div), none
+    # adds nothing.  Its gradient is p sum pi - pi with p = 0.  A cell that is not legal is not looked at at all.
+    from alphazero_amd import policy
+
+    rows, last = 6, actions - 1
+    g = torch.Generator().manual_seed(actions)
+    x = torch.randn(rows, actions, generator=g)
+    pi = torch.rand(rows, actions, generator=g)
+    pi /= pi.sum(1, keepdim=True)
+    legal = torch.ones(rows, actions, dtype=torch.bool)
+    x[0, last] = -math.inf                                 # a target that cannot be reached
+    x[1, 1], pi[1, 1] = -math.inf, 0.0                     # the same without a target
+    legal[2, last], x[2, last], pi[2, last] = False, -math.inf, 0.5
+    x[3] = -math.inf                                       # every legal cell
+    x[4], pi[4] = -math.inf, 0.0
+    legal[5] = False                                       # a full board
+    x = x.to(dtype)
+    xg = x.cuda().requires_grad_()
+    v = torch.zeros(rows, device="cuda")
+    parts = [policy.loss(xg[i:i + 1], v[:1], pi[i:i + 1].cuda(), v[:1], legal=legal[i:i + 1].cuda(), parts=True)[1].item()
+             for i in range(rows)]
+    total = policy.loss(xg, v, pi.cuda(), v, legal=legal.cuda())
+    dx, = torch.autograd.grad(total, xg)
+    logp, p, d, logS = _exact(x, legal)
+    q = torch.where(legal, pi.double(), 0.0)
+    terms = torch.where(q > 0, q * (torch.log(q) - logp), 0.0)
+    tS = _sum_tol(p, d, logS, actions)
+    dd = torch.where((q > 0) & legal & (d > -math.inf), d.abs(), 0.0)
+    mag = torch.where(q > 0, q * (torch.log(q).abs() + dd + logS + 1), 0.0)
+    tol = (q * (tS + 3 * (dd + logS) * U) + mag * (8 + actions / 64) * U).sum(1)
+    _ok(torch.tensor(parts), terms.sum(1), tol + terms.sum(1).nan_to_num(posinf=0.0).abs() * U, "parts")
+    assert [math.isinf(t) for t in parts] == [True, False, False, True, False, False] and total.item() == math.inf
+    assert parts[4] == 0 and parts[5] == 0
+    W = q.sum(1, keepdim=True)
+    wx = torch.where(legal, p * W - q, 0.0) / rows
+    t = (p * W * ((4 * dd + 24 + actions / 32) * U + tS) + 4 * U * (p * W + q)) / rows
+    t = t + (wx.abs() + t) * torch.finfo(dtype).eps / 2 + (2.0 ** -25 if dtype == torch.float16 else 0)
+    _ok(dx, wx, t, "d_logits")
+    assert not dx[5].any() and dx[2, last] == 0
+
+
+@pytest.mark.parametrize("actions", [9, 225, 3000])
+def test_loss_of_the_smallest_targets(actions):
+    # subnormal float32 targets (a softmax far from its peak) count for what they are
+    from alphazero_amd import policy
+
+    g = torch.Generator().manual_seed(actions)
+    x = torch.randn(3, actions, generator=g)
+    pi = torch.softmax(torch.randn(3, actions, generator=g), 1)
+    tiny = torch.tensor([2.0 ** -149, 1e-42, 1e-39, 2.0 ** -126])
+    pi[0, :4] = tiny                                       # among ordinary ones
+    pi[1] = tiny[torch.randint(0, 4, (actions,), generator=g)]  # and alone
+    v = torch.zeros(3, device="cuda")
+    parts = torch.stack([policy.loss(x[i:i + 1].cuda(), v[:1], pi[i:i + 1].cuda(), v[:1], parts=True)[1] for i in range(3)])
+    logp, p, d, logS = _exact(x, torch.ones_like(x, dtype=torch.bool))
+    q = pi.double()
+    terms = q * (torch.log(q) - logp)
+    tS = _sum_tol(p, d, logS, actions)
+    mag = q * (torch.log(q).abs() + logp.abs() + 1)
+    tol = (q * (tS + 3 * (d.abs() + logS) * U) + mag * (8 + actions / 64) * U).sum(1) + 2 * actions * 2.0 ** -149
+    _ok(parts, terms.sum(1), tol + terms.sum(1).abs() * U, "parts")
