@@ -485,11 +485,14 @@ int az_policy_loss(int n, int actions, const void *d_logits, int dtype, long lon
  * AZ_BF16 / AZ_F16): X = G / |G|_F, then `steps` times X <- a X + (b A + c A^2) X with A = X X' (X' X for a matrix taller
  * than wide) and (a, b, c) = (3.4445, -4.7750, 2.0315), to d_out[i] [rows][ld_out] in the same type (d_out[i] may be
  * d_in[i]; outputs overlap nothing else).  A matrix of zeros stays zero, one with an infinity or NaN becomes NaN.  The
- * products have float32 precision whatever the type, and a result is rounded to its type once; the same call gives the same
+ * products have float32 precision whatever the type, relative to the whole matrix, and a result is rounded to its type once:
+ * numbers are held to 22 bits, but not below 2^-39 of |G| (in Q: 2^-35 of 1), so a row far smaller than |G| keeps fewer
+ * digits (a row of 1e-5 |G| five, of 1e-7 |G| three, of 1e-11 |G| none).  A step multiplies what is missing by up to a; the
+ * limit of 10 steps keeps the result as a whole as good as float32 products make it.  The same call gives the same
  * bits (how many matrices there are decides how sums are split, so a matrix alone may differ in the last bits).  d_work:
  * az_muon_work(count, rows, cols) bytes (0 for small matrices), used by this call only; the device current at the call is
  * the one of the pointers and of `stream`. */
-enum { AZ_MUON_MAX_DIM = 32768, AZ_MUON_MAX_CELLS = 1 << 28, AZ_MUON_MAX_STEPS = 20 };
+enum { AZ_MUON_MAX_DIM = 32768, AZ_MUON_MAX_CELLS = 1 << 28, AZ_MUON_MAX_STEPS = 10 };
 long long az_muon_work(int count, int rows, int cols);
 int az_muon_orthogonalise(int count, int rows, int cols, const void *const *d_in, long long ld_in, void *const *d_out,
                           long long ld_out, int dtype, int steps, void *d_work, void *stream);

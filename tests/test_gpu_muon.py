@@ -346,3 +346,33 @@ def test_low_rank_updates_in_16_bits(shape, dtype, rank, floor):
     g = g.to(dtype).cuda()
     for steps in (3, 4, 5, 6, 7):
         _check(muon.orthogonalise(g, steps), g, steps)
+
+
+@pytest.mark.parametrize("shape", [(30, 600), (64, 576), (2, 60, 200), (130, 1000), (256, 2304), (2, 400, 2000), (2, 1024, 4096)])
+@pytest.mark.parametrize("rows", ["one", "half", "spread"])
+def test_updates_with_rows_of_very_different_size(shape, rows):
+    # A nearly dead channel.  Numbers of X stop at 2^-39 (an error of 2^-40 each), of A at 2^-38, of Q at 2^-34 (2^-35 each,
+    # with A's 2^-39 times b and c: at most 2^-34), so a step adds to each row at most 2^-40 sqrt(n) + 2^-34 |X|, and
+    # later steps multiply that by at most a each: sqrt(m) (...) a^(steps - 1) sum_k a^-k, the sum being below 1.41.  To that
+    # come 16 u a step for the products (8 u, and as much again for the errors' mutual growth).
+    from alphazero_amd import muon
+
+    m, n = shape[-2:]
+    for s in (1e-3, 1e-5, 1e-7, 1e-9, 1e-11):
+        g = _updates(shape, 41, 1.0)
+        if rows == "one":
+            g[..., m // 3, :] *= s
+        elif rows == "half":
+            g[..., ::2, :] *= s
+        else:
+            g *= s ** (torch.arange(m) / m).unsqueeze(1)
+        for steps in (1, 5, 10) if m < 400 else (5, 10):
+            x = g.double().cuda()  # (the definition on the GPU, in 64 bits)
+            x = x / x.square().sum((-1, -2), keepdim=True).sqrt()
+            for _ in range(steps):
+                A = x @ x.transpose(-1, -2).contiguous()
+                x = ABC[0] * x + (ABC[1] * A + ABC[2] * (A @ A)) @ x
+            off = (muon.orthogonalise(g.cuda(), steps).double() - x).flatten(-2).norm(dim=-1)
+            size = x.flatten(-2).norm(dim=-1)
+            tol = 16 * steps * U * size + 1.41 * ABC[0] ** (steps - 1) * m ** 0.5 * (2.0 ** -40 * n ** 0.5 + 2.0 ** -34 * size)
+            assert (off <= tol).all(), (s, steps, off, tol)

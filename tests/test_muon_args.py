@@ -71,3 +71,13 @@ def test_workspace_grows_with_the_batch_and_ends():
     for shape in ((100, 400), (1000, 1000), (70, 20000)):
         assert L.az_muon_work(100000, *shape) <= (1 << 30) + 4096
     assert L.az_muon_work(3, 16384, 16384) > 0
+
+
+def test_steps_end_where_the_precision_does():
+    for steps in (11, 20):
+        with pytest.raises(ValueError, match="steps must be 1..10"):
+            muon.orthogonalise(G, steps)
+        with pytest.raises(ValueError, match="steps must be 1..10"):
+            muon.Muon([torch.nn.Parameter(torch.zeros(3, 3))], steps=steps)
+        one = (C.c_void_p * 1)(0x1000)
+        assert E.load_library().az_muon_orthogonalise(1, 4, 9, one, 9, one, 9, 0, steps, None, None) == E.ERR_ARG
