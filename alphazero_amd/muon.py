@@ -101,7 +101,10 @@ class Muon(torch.optim.Optimizer):
     biases and batch-norm parameters to another optimiser, `weights_of` tells them apart):
 
         m <- momentum m + g,   u = g + momentum m (nesterov) or m,
-        w <- w (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) orthogonalise(u)"""
+        w <- w (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) orthogonalise(u)
+
+    Whatever the weights' type, m and u are float32 and a step is rounded into the weight once: in 16 bits a momentum of 0.999
+    would not decay at all, and one of 0.95 would stop at gradients below 6e-7."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5):
         if lr < 0 or not 0 <= momentum < 1 or weight_decay < 0:
@@ -127,6 +130,20 @@ class Muon(torch.optim.Optimizer):
         params = list(module.parameters())
         return [p for p in params if p.dim() >= 2], [p for p in params if p.dim() < 2]
 
+    def load_state_dict(self, state_dict):
+        loaded = []
+        hook = self.register_load_state_dict_pre_hook(lambda _, state: loaded.append(state))  # (as other hooks leave it)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            hook.remove()
+        # the base class gives what it loads the weight's type: m again, in float32
+        numbers = [i for group in loaded[-1]["param_groups"] for i in group["params"]]
+        for i, p in zip(numbers, (p for group in self.param_groups for p in group["params"])):
+            m = loaded[-1]["state"].get(i, {}).get("momentum")
+            if m is not None:
+                self.state[p]["momentum"] = m.detach().to(p.device, torch.float32, copy=True)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -137,19 +154,23 @@ class Muon(torch.optim.Optimizer):
             params = [p for p in group["params"] if p.grad is not None and p.numel()]
             if not params:
                 continue
-            grads = [p.grad for p in params]
-            for p in params:
+            grads = [p.grad.float() for p in params]  # (float32 ones are these themselves, and so are the weights below)
+            for p, g in zip(params, grads):
                 if "momentum" not in self.state[p]:
-                    self.state[p]["momentum"] = torch.zeros_like(p.grad)
+                    self.state[p]["momentum"] = torch.zeros_like(g)
             moments = [self.state[p]["momentum"] for p in params]
             mu = group["momentum"]
             torch._foreach_mul_(moments, mu)
             torch._foreach_add_(moments, grads)
             updates = torch._foreach_add(grads, moments, alpha=mu) if group["nesterov"] else moments
             updates = orthogonalise(updates, group["steps"])
+            weights = [p.float() for p in params]
             if group["weight_decay"]:
-                torch._foreach_mul_(params, 1 - group["lr"] * group["weight_decay"])
+                torch._foreach_mul_(weights, 1 - group["lr"] * group["weight_decay"])
             factors = [-group["lr"] * max(1.0, p.shape[0] * p.shape[0] / p.numel()) ** 0.5 for p in params]
             torch._foreach_mul_(updates, factors)
-            torch._foreach_add_(params, updates)
+            torch._foreach_add_(weights, updates)
+            for p, w in zip(params, weights):
+                if w is not p:
+                    p.copy_(w)
         return loss

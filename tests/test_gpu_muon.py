@@ -376,3 +376,86 @@ def test_updates_with_rows_of_very_different_size(shape, rows):
             size = x.flatten(-2).norm(dim=-1)
             tol = 16 * steps * U * size + 1.41 * ABC[0] ** (steps - 1) * m ** 0.5 * (2.0 ** -40 * n ** 0.5 + 2.0 ** -34 * size)
             assert (off <= tol).all(), (s, steps, off, tol)
+
+
+@pytest.mark.parametrize("dtype,momentum,quiet,size", [(torch.float16, 0.95, 16, 6e-7), (torch.bfloat16, 0.999, 250, 1e-7), (torch.float32, 0.95, 16, 1e-7)])
+def test_momentum_of_16_bit_weights_decays(dtype, momentum, quiet, size):
+    # A gradient, a number of steps without one, another gradient: how much of the first is left decides the direction.  In 16
+    # bits 0.95 m rounds back to m below 6e-7 (float16), and 0.999 m everywhere (bfloat16).
+    from alphazero_amd import muon
+
+    gen = torch.Generator().manual_seed(51)
+    first, second = [(torch.randn(24, 60, generator=gen) * size).to(dtype) for _ in range(2)]
+    w = torch.nn.Parameter(torch.zeros(24, 60, dtype=dtype, device="cuda"))
+    opt = muon.Muon([w], lr=0.02, momentum=momentum)
+    m, none = torch.zeros(24, 60, dtype=torch.float64), torch.zeros_like(first)
+    for g in [first] + [none] * quiet + [second]:
+        w.grad = g.cuda()
+        w.data.zero_()
+        opt.step()
+        m = momentum * m + g.double()
+    u = _exact(g.double() + momentum * m)
+    want = -0.02 * u
+    # the last step alone: the update's own error (float32 products, momentum in float32: quiet u), half a step of the weight
+    off = (w.detach().cpu().double() - want).norm()
+    assert off <= 0.02 * ABC[0] ** 4 * 1.41 * (32 + 2 * quiet) * U + torch.finfo(dtype).eps / 2 * want.norm()
+
+
+TYPES_16 = [torch.bfloat16, torch.float16]
+
+
+@pytest.mark.parametrize("dtype", TYPES_16)
+def test_weights_of_16_bits_step_by_step(dtype):
+    # several weights of both kinds in one optimiser: each step is computed in float32 and rounded into the weight once
+    from alphazero_amd import muon
+
+    gen = torch.Generator().manual_seed(52)
+    shapes = [(16, 4, 3, 3), (40, 10), (130, 300)]
+    w = [torch.nn.Parameter(torch.randn(*s, generator=gen).to(t).cuda()) for s in shapes for t in (dtype, torch.float32)]
+    opt = muon.Muon(w, lr=0.05, momentum=0.9, weight_decay=0.02)
+    moments = [torch.zeros(p.shape, dtype=torch.float64) for p in w]
+    for _ in range(3):
+        for i, p in enumerate(w):
+            g = (torch.randn(p.shape, generator=gen) * 1e-3).to(p.dtype)
+            p.grad = g.cuda()
+            moments[i] = 0.9 * moments[i] + g.double()
+        before = [p.detach().cpu().double() for p in w]
+        opt.step()
+        for i, (p, b) in enumerate(zip(w, before)):
+            u = _exact((p.grad.cpu().double() + 0.9 * moments[i]).flatten(1)).view(p.shape)
+            want = b * (1 - 0.05 * 0.02) - 0.05 * max(1.0, p.shape[0] / p[0].numel()) ** 0.5 * u
+            off = (p.detach().cpu().double() - want).abs()
+            # 1e-5 of the step for the update (as above), 3 u for decay, product and sum, half a step of the weight
+            assert (off <= 1e-5 * 0.05 * u.norm() + want.abs() * (torch.finfo(p.dtype).eps / 2 + 3 * U) +
+                    (2.0 ** -25 if p.dtype == torch.float16 else 0)).all()
+        assert all(opt.state[p]["momentum"].dtype == torch.float32 for p in w)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32] + TYPES_16)
+def test_optimiser_goes_on_from_its_saved_state(dtype):
+    import io
+
+    from alphazero_amd import muon
+
+    gen = torch.Generator().manual_seed(53)
+    grads = [(torch.randn(20, 50, generator=gen) * 1e-6).to(dtype).cuda() for _ in range(6)]
+
+    def steps(w, opt, some):
+        for g in some:
+            w.grad = g.clone()
+            opt.step()
+
+    a = torch.nn.Parameter(torch.zeros(20, 50, dtype=dtype, device="cuda"))
+    one = muon.Muon([a], lr=0.1, momentum=0.9)
+    steps(a, one, grads[:3])
+    b = torch.nn.Parameter(a.detach().clone())
+    two = muon.Muon([b], lr=0.5)
+    file = io.BytesIO()
+    torch.save(one.state_dict(), file)
+    file.seek(0)
+    two.load_state_dict(torch.load(file, weights_only=True, map_location="cpu"))
+    assert two.param_groups[0]["momentum"] == 0.9 and two.state[b]["momentum"].dtype == torch.float32
+    assert torch.equal(two.state[b]["momentum"], one.state[a]["momentum"])
+    steps(a, one, grads[3:])
+    steps(b, two, grads[3:])
+    assert torch.equal(a, b) and two.state[b]["momentum"].data_ptr() != one.state[a]["momentum"].data_ptr()
