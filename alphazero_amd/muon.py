@@ -30,7 +30,7 @@ def _check(rows, cols, dtype, steps):
 
 def _on_gpu(tensors):
     if any(not t.is_cuda for t in tensors):
-        _refuse("updates must be on a GPU (there is no CPU path)")
+        _refuse("weights and updates must be on a GPU (there is no CPU path)")
 
 
 def _run(inputs, outputs, rows, cols, ld, dtype, device, steps):
@@ -96,6 +96,15 @@ def orthogonalise(updates, steps=5):
     return outs
 
 
+def _check_options(group, read=True):
+    """read=False: a learning rate that is a tensor is not looked at (that would wait for the GPU)."""
+    lr, decay = group["lr"], group["weight_decay"]
+    if (read or not torch.is_tensor(lr)) and not lr >= 0 or not decay >= 0 or not 0 <= group["momentum"] < 1:
+        _refuse("lr and weight_decay must not be negative, momentum must be in [0, 1)")
+    if not isinstance(group["steps"], int) or not 1 <= group["steps"] <= MAX_STEPS:
+        _refuse(f"steps must be 1..{MAX_STEPS}")
+
+
 class Muon(torch.optim.Optimizer):
     """Momentum with orthogonalised updates, for weights of two or more dimensions (convolutions and dense layers; give
     biases and batch-norm parameters to another optimiser, `weights_of` tells them apart):
@@ -107,15 +116,14 @@ class Muon(torch.optim.Optimizer):
     would not decay at all, and one of 0.95 would stop at gradients below 6e-7."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5):
-        if lr < 0 or not 0 <= momentum < 1 or weight_decay < 0:
-            _refuse("lr and weight_decay must not be negative, momentum must be in [0, 1)")
-        if not isinstance(steps, int) or not 1 <= steps <= MAX_STEPS:
-            _refuse(f"steps must be 1..{MAX_STEPS}")
-        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps))
+        options = dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps)
+        _check_options(options)
+        super().__init__(params, options)
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
         try:
+            _check_options(self.param_groups[-1])
             for p in self.param_groups[-1]["params"]:
                 if p.dim() < 2:
                     _refuse("Muon takes weights of two or more dimensions")
@@ -150,8 +158,16 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for group in self.param_groups:
-            params = [p for p in group["params"] if p.grad is not None and p.numel()]
+        groups = [(group, [p for p in group["params"] if p.grad is not None and p.numel()]) for group in self.param_groups]
+        for group, params in groups:  # what is refused is refused before anything has changed
+            _check_options(group, read=False)
+            for p in params:
+                if p.grad.layout != torch.strided:
+                    _refuse("Muon takes no sparse gradients")
+                if p.dtype not in TYPES:
+                    _refuse(f"weights must be float32, bfloat16 or float16, not {p.dtype}")
+            _on_gpu(params)
+        for group, params in groups:
             if not params:
                 continue
             grads = [p.grad.float() for p in params]  # (float32 ones are these themselves, and so are the weights below)

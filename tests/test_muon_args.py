@@ -81,3 +81,34 @@ def test_steps_end_where_the_precision_does():
             muon.Muon([torch.nn.Parameter(torch.zeros(3, 3))], steps=steps)
         one = (C.c_void_p * 1)(0x1000)
         assert E.load_library().az_muon_orthogonalise(1, 4, 9, one, 9, one, 9, 0, steps, None, None) == E.ERR_ARG
+
+
+def test_optimiser_checks_the_options_of_every_group():
+    opt = muon.Muon([torch.nn.Parameter(torch.zeros(3, 3))])
+    for bad in (dict(lr=-1.0), dict(momentum=1.0), dict(momentum=-0.1), dict(weight_decay=-0.1), dict(steps=0), dict(lr=float("nan"))):
+        with pytest.raises(ValueError):
+            opt.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(2, 2))], **bad))
+        with pytest.raises(ValueError):
+            muon.Muon([dict(params=[torch.nn.Parameter(torch.zeros(2, 2))], **bad)])
+        assert len(opt.param_groups) == 1
+
+
+def test_a_refused_step_changes_nothing():
+    # no path on the CPU, an option changed to one that is refused, gradients of a kind that is not taken
+    def weight(grad=None):
+        p = torch.nn.Parameter(torch.ones(3, 3))
+        p.grad = torch.ones(3, 3) if grad is None else grad
+        return p
+
+    ok, late = weight(), weight()
+    opt = muon.Muon([dict(params=[ok]), dict(params=[late])], lr=0.1, weight_decay=0.1)
+    for i, change in ((0, {}), (1, dict(steps=11)), (1, dict(momentum=1.0)), (1, dict(lr=-1.0))):
+        kept = dict(opt.param_groups[i])
+        opt.param_groups[i].update(change)
+        with pytest.raises(ValueError):
+            opt.step()
+        opt.param_groups[i].update(kept)
+        assert not opt.state[ok] and not opt.state[late]
+        assert torch.equal(ok.detach(), torch.ones(3, 3)) and torch.equal(late.detach(), torch.ones(3, 3))
+    with pytest.raises(ValueError, match="sparse"):
+        muon.Muon([weight(torch.ones(3, 3).to_sparse())]).step()
