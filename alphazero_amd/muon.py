@@ -9,7 +9,7 @@ import functools
 import torch
 
 from . import engine as _E
-from .policy import TYPES, _call, _ptr, _refuse
+from .policy import TYPES, _call, _ptr, _refuse, _untraced
 
 MAX_DIM, MAX_CELLS, MAX_STEPS = 32768, 1 << 28, 10  # AZ_MUON_MAX_*
 
@@ -63,6 +63,7 @@ def orthogonalise(updates, steps=5):
     Whatever the type, the steps are computed with products of float32 precision, relative to the whole matrix, and rounded
     once at the end.  Numbers below 2^-39 of |G| are not kept: a row of 1e-5 |G| comes out with five digits, one of 1e-7 |G|
     with three, one of 1e-11 |G| as zero."""
+    _untraced("muon.orthogonalise")
     if torch.is_tensor(updates):
         if updates.dim() not in (2, 3):
             _refuse("updates must be a matrix, a batch of matrices or a list of tensors")

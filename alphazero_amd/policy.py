@@ -13,6 +13,7 @@ import functools
 from collections import namedtuple
 
 import torch
+from torch.autograd import forward_ad as _forward
 
 from . import engine as _E
 
@@ -22,6 +23,7 @@ SHORT_MAX = 1024  # rows up to here are held in registers
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # AZ_F32, AZ_BF16, AZ_F16
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+_tracing = getattr(torch._C, "_get_tracing_state", None) or (lambda: torch.jit.is_tracing() or None)
 
 Score = namedtuple("Score", "logp entropy top_moves top_logp")
 
@@ -62,6 +64,17 @@ def _loss_work(n, actions):
 def _once():
     if torch.is_grad_enabled():  # a backward pass that builds a graph of itself
         raise RuntimeError("the policy operators can be differentiated once (no create_graph)")
+
+
+def _untraced(what):
+    if _tracing() is not None:  # a trace would hold the addresses of this call's tensors, or none of its work
+        raise RuntimeError(f"{what} cannot be traced")
+
+
+def _without_tangents(*tensors):
+    for t in tensors:
+        if torch.is_tensor(t) and _forward.unpack_dual(t).tangent is not None:
+            raise RuntimeError("the policy operators have no forward-mode derivative")
 
 
 def _on_one_gpu(logits, *others):
@@ -179,7 +192,10 @@ def score(logits, moves=None, *, board=None, legal=None, top=0):
               (-1 where no legal move is left) and float32 top_logp (-inf there).  0: both are None
     entropy   float32 [n], of the distribution over the legal moves
 
-    logp and entropy are differentiable for logits (once); the alternatives are not."""
+    logp and entropy are differentiable for logits (once, in reverse mode); the alternatives are not."""
+    _untraced("policy.score")
+    if _forward._current_level >= 0:  # (within a dual_level; no other call pays for the look)
+        _without_tangents(logits)
     logits, board, legal, rows = _rows(logits, board, legal)
     n = rows[0]
     if moves is not None:
@@ -248,8 +264,11 @@ def loss(logits, value, pi, r, *, board=None, legal=None, parts=False):
     pi      float32 [n, actions], targets (rows need not sum to 1; masked cells are not looked at, a target on a legal cell
             at -inf makes the loss infinite);  r  float32, n results
 
-    Differentiable (once) for logits and value.  parts=True returns (total, policy part, value part), the parts without
+    Differentiable (once, in reverse mode) for logits and value.  parts=True returns (total, policy part, value part), the parts without
     gradient.  Zero records give 0."""
+    _untraced("policy.loss")
+    if _forward._current_level >= 0:
+        _without_tangents(logits, value, pi, r)
     logits, board, legal, rows = _rows(logits, board, legal)
     n, actions = rows[:2]
     if value.dtype not in (torch.float32, logits.dtype) or value.numel() != n:

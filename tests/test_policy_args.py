@@ -69,3 +69,29 @@ def test_c_entries_refuse():
     assert L.az_policy_score_work(4, 400, 8) == 0 and L.az_policy_score_work(4, 4000, 8) > 0
     assert L.az_policy_score_work(-1, 400, 8) == -1 and L.az_policy_loss_work(1, 0) == -1
     assert [L.az_policy_mask_words(a) for a in (0, 1, 64, 65, 1024, 1025)] == [0, 1, 1, 2, 16, 0]
+
+
+def test_forward_mode_derivatives_are_refused():
+    # a tangent would be lost without a word, with and without grad mode
+    import torch.autograd.forward_ad as fw
+
+    with fw.dual_level():
+        x, v, pi, r = (fw.make_dual(t, torch.ones_like(t)) for t in (X, V, PI, R))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    policy.score(x)
+                for args in ((x, V, PI, R), (X, v, PI, R), (X, V, pi, R), (X, V, PI, r)):
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        policy.loss(*args)
+        with pytest.raises(ValueError, match="no CPU path"):  # (nothing to lose)
+            policy.score(X)
+
+
+def test_traces_are_refused():
+    # a trace keeps addresses, not tensors: its result on other inputs would be the first call's, or freed memory's
+    from alphazero_amd import muon
+
+    for f, args in ((policy.score, (X,)), (policy.loss, (X, V, PI, R)), (muon.orthogonalise, (X,))):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(f, args)
