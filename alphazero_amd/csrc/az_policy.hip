@@ -571,11 +571,11 @@ __device__ __forceinline__ void rebase(float &S, float &U, float from, float to)
     S = s;
 }
 
-template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_parts(Rows a, Chunks c, LongOut o)
+template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_parts(Rows a, Chunks c, LongOut o, long long first)
 {
     if (o.unless_one && *o.unless_one == 1.f) return;
     const int lane = threadIdx.x & 63;
-    const long long unit = (long long)blockIdx.x * WAVES + wave_of();
+    const long long unit = (first + blockIdx.x) * WAVES + wave_of();
     if (unit >= (long long)a.n * c.count) return;
     const long long row = unit / c.count;
     const int chunk = (int)(unit - row * c.count);
@@ -662,11 +662,11 @@ __device__ __forceinline__ Part join_parts(const Part *part, int count, int lane
 
 // one workgroup per row: outputs of az_policy_score from the chunks' numbers and lists.  The lists are merged in LDS: a
 // lane holds the heads of every 64th list, each round takes the largest head (of equal ones the lowest index)
-template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_score(Rows a, Chunks c, LongOut w, ScoreOut o)
+template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_score(Rows a, Chunks c, LongOut w, ScoreOut o, long long first)
 {
     extern __shared__ float s_list[]; // [chunks][top] values, then indices
     const int lane = threadIdx.x;
-    const long long row = blockIdx.x;
+    const long long row = first + blockIdx.x;
     const int cells = c.count * o.top;
     int *s_index = (int *)(s_list + cells);
     for (int i = lane; i < cells; i += 64 * WAVES * 4) { // four loads in flight per thread
@@ -759,10 +759,10 @@ template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_score(Ro
     }
 }
 
-template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_score_grad(Rows a, Chunks c, ScoreGrad o)
+template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_score_grad(Rows a, Chunks c, ScoreGrad o, long long first)
 {
     const int lane = threadIdx.x & 63;
-    const long long unit = (long long)blockIdx.x * WAVES + wave_of();
+    const long long unit = (first + blockIdx.x) * WAVES + wave_of();
     if (unit >= (long long)a.n * c.count) return;
     const long long row = unit / c.count;
     const int chunk = (int)(unit - row * c.count);
@@ -866,6 +866,14 @@ int grid_of(long long units)
     return (int)(b < GRID_MAX ? b : GRID_MAX);
 }
 
+// A launch counts its threads in 32 bits, so workgroups without end come in several launches: f(first, how many)
+constexpr long long LAUNCH_MAX = 1ll << 23;
+template <class F> void in_launches(long long groups, F f)
+{
+    for (long long first = 0; first < groups; first += LAUNCH_MAX)
+        f(first, dim3((unsigned)(groups - first < LAUNCH_MAX ? groups - first : LAUNCH_MAX)));
+}
+
 // Chunks of a long row: about 8192 wavefronts over all rows (32 per CU) when the rows alone are fewer, chunks of at least
 // one step, at most as many as one wavefront can merge (their lists in 32 KB of LDS).
 Chunks chunks_of(int n, int A, int top)
@@ -879,6 +887,9 @@ Chunks chunks_of(int n, int A, int top)
     const long long len = ((A + want - 1) / want + LONG_STEP - 1) / LONG_STEP * LONG_STEP;
     return Chunks{(int)len, (int)((A + len - 1) / len)};
 }
+
+// workgroups with a wavefront for each chunk
+long long groups_of(int n, const Chunks &c) { return ((long long)n * c.count + WAVES - 1) / WAVES; }
 
 bool rows_ok(const Rows &a, int dtype)
 {
@@ -956,12 +967,14 @@ int az_policy_score(int n, int actions, const void *d_logits, int dtype, long lo
     w.list_v = (float *)(w.part + (size_t)n * c.count);
     w.list_i = (int *)(w.list_v + (size_t)n * c.count * top);
     w.top = top;
-    const long long units = (long long)n * c.count;
-    if ((units + WAVES - 1) / WAVES > 0x7fffffffll) return AZ_ERR_ARG;
     by_type(dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        hipLaunchKernelGGL((k_long_parts<T>), dim3((unsigned)((units + WAVES - 1) / WAVES)), block, 0, st, a, c, w);
-        hipLaunchKernelGGL((k_long_score<T>), dim3(n), block, (size_t)c.count * top * 8, st, a, c, w, o);
+        in_launches(groups_of(n, c), [&](long long first, dim3 grid) {
+            hipLaunchKernelGGL((k_long_parts<T>), grid, block, 0, st, a, c, w, first);
+        });
+        in_launches(n, [&](long long first, dim3 grid) {
+            hipLaunchKernelGGL((k_long_score<T>), grid, block, (size_t)c.count * top * 8, st, a, c, w, o, first);
+        });
     });
     return launch_ok();
 }
@@ -981,8 +994,6 @@ int az_policy_score_grad(int n, int actions, const void *d_logits, int dtype, lo
     const dim3 block(64 * WAVES);
     const hipStream_t st = (hipStream_t)stream;
     const Chunks c = chunks_of(n, actions, 0);
-    const long long units = (long long)n * c.count;
-    if (actions > SHORT_MAX && (units + WAVES - 1) / WAVES > 0x7fffffffll) return AZ_ERR_ARG;
     by_type(dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
         if (actions <= SHORT_MAX)
@@ -990,7 +1001,9 @@ int az_policy_score_grad(int n, int actions, const void *d_logits, int dtype, lo
                 hipLaunchKernelGGL((k_score_grad<T, decltype(w)::value>), dim3(grid_of(n)), block, 0, st, a, o);
             });
         else
-            hipLaunchKernelGGL((k_long_score_grad<T>), dim3((unsigned)((units + WAVES - 1) / WAVES)), block, 0, st, a, c, o);
+            in_launches(groups_of(n, c), [&](long long first, dim3 grid) {
+                hipLaunchKernelGGL((k_long_score_grad<T>), grid, block, 0, st, a, c, o, first);
+            });
     });
     return launch_ok();
 }
@@ -1025,16 +1038,16 @@ int az_policy_loss(int n, int actions, const void *d_logits, int dtype, long lon
         });
     } else {
         const Chunks c = chunks_of(n, actions, 0);
-        const long long units = (long long)n * c.count;
-        if ((units + WAVES - 1) / WAVES > 0x7fffffffll) return AZ_ERR_ARG;
         LongOut w = {};
         w.part = (Part *)((char *)d_work + GRID_MAX * 2 * sizeof(double));
         w.pi = d_pi;
         w.unless_one = only_if_scaled ? d_scale : nullptr;
-        blocks = grid_of(units);
+        blocks = grid_of((long long)n * c.count);
         by_type(dtype, [&](auto *t) {
             using T = std::remove_pointer_t<decltype(t)>;
-            hipLaunchKernelGGL((k_long_parts<T>), dim3((unsigned)((units + WAVES - 1) / WAVES)), block, 0, st, a, c, w);
+            in_launches(groups_of(n, c), [&](long long first, dim3 grid) {
+                hipLaunchKernelGGL((k_long_parts<T>), grid, block, 0, st, a, c, w, first);
+            });
             hipLaunchKernelGGL((k_long_loss<T>), dim3(blocks), block, 0, st, a, c, (const Part *)w.part, o);
         });
     }

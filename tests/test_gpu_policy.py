@@ -511,3 +511,47 @@ def test_loss_of_the_smallest_targets(actions):
     mag = q * (torch.log(q).abs() + logp.abs() + 1)
     tol = (q * (tS + 3 * (d.abs() + logS) * U) + mag * (8 + actions / 64) * U).sum(1) + 2 * actions * 2.0 ** -149
     _ok(parts, terms.sum(1), tol + terms.sum(1).abs() * U, "parts")
+
+
+def test_more_long_rows_than_a_launch_has_workgroups():
+    # 2^24 workgroups of 256 threads are one thread too many for a launch; the rows around the seams are the ones that differ
+    from alphazero_amd import policy
+
+    n, a = (1 << 24) + 5, 1025
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 180 << 30:
+        pytest.skip("180 GiB of free GPU memory needed")
+    g = torch.Generator().manual_seed(6)
+    at = torch.tensor([0, 1, (1 << 23) - 1, 1 << 23, (1 << 23) + 1, (1 << 24) - 1, 1 << 24, n - 1])
+    some = torch.randn(len(at), a, generator=g).half()
+    moves = torch.zeros(n, dtype=torch.int32, device="cuda")
+    moves[at.cuda()] = torch.arange(1, 9, dtype=torch.int32, device="cuda") * 100
+    x = torch.zeros(n, a, dtype=torch.float16, device="cuda")
+    x[at.cuda()] = some.cuda()
+    rest = torch.ones(n, dtype=torch.bool, device="cuda")
+    rest[at.cuda()] = False
+    x.requires_grad_()
+    s = policy.score(x, moves, top=2)
+    logp, p, d, logS = _exact(some, torch.ones_like(some, dtype=torch.bool))
+    tS = _sum_tol(p, d, logS, a).squeeze(1)
+    mine = (torch.arange(8), torch.arange(1, 9) * 100)
+    _ok(s.logp[at.cuda()], logp[mine], tS + 3 * (d[mine].abs() + logS.squeeze(1)) * U, "logp")
+    assert torch.equal(s.top_moves[at.cuda(), 0].cpu().long(), some.argmax(1))
+    assert ((s.logp[rest] + math.log(a)).abs() <= 40 * U).all() and ((s.entropy[rest] - math.log(a)).abs() <= 80 * U).all()
+    assert (s.top_moves[rest] == torch.tensor([0, 1], device="cuda")).all()
+    dx, = torch.autograd.grad(s.logp, x, torch.ones(n, device="cuda"))
+    want = -p
+    want[mine] += 1
+    _ok(dx[at.cuda()], want, want.abs() * (2.0 ** -11 + 60 * U) + 60 * U * p + 2.0 ** -25, "d_logits")
+    ends = dx[rest][:: 1 << 18]
+    assert ((ends[:, 0].float() - 1024 / 1025).abs() <= 2.0 ** -11).all() and ((ends[:, 1:].float() + 1 / 1025).abs() <= 2.0 ** -21).all()
+    del dx, ends, s
+    x = x.detach()
+    pi = torch.zeros(n, a, device="cuda")
+    pi[at.cuda(), moves[at.cuda()].long()] = 1.0
+    v = torch.zeros(n, device="cuda")
+    got = policy.loss(x, v, pi, v).double() * n
+    off = (got.cpu() + logp[mine].sum()).abs()
+    assert off <= (tS + 3 * (d[mine].abs() + logS.squeeze(1)) * U).sum() + 4 * U * logp[mine].sum().abs()
+    del x, pi
+    torch.cuda.empty_cache()
