@@ -127,13 +127,29 @@ def _rows(logits, board, legal):
     return logits, board, legal, (n, actions, logits.data_ptr(), kind, ld, at_board, at_legal, ld_legal)
 
 
-def _saved(rows, logits, board, legal):
-    """Tensors that come back from autograd and the entry points' leading arguments, made again where a saved-tensor hook
-    has moved a tensor."""
-    if logits.data_ptr() == rows[2] and _ptr(board) == rows[5] and _ptr(legal) == rows[6] and \
-            (rows[0] <= 1 or (logits.stride(0) == rows[4] and (legal is None or legal.stride(0) == rows[7]))):
-        return logits, board, legal, rows
-    return _rows(logits, board, legal)
+def _keep(ctx, rows, device, logits, board, legal, *others):
+    """Saves tensors for the backward pass (the others dense)."""
+    ctx.rows, ctx.device = rows, device
+    ctx.kept = [None if t is None else (t.data_ptr(), t.shape, t.dtype) for t in others]
+    ctx.save_for_backward(logits, board, legal, *others)
+
+
+def _kept(ctx):
+    """What _keep saved: the entry points' leading arguments, and the tensors.  A saved-tensor hook may have moved a tensor or
+    laid it out otherwise; one that hands back other sizes or types, or a tensor on another device, is refused."""
+    logits, board, legal, *others = ctx.saved_tensors
+    rows = ctx.rows
+    if not (logits.data_ptr() == rows[2] and _ptr(board) == rows[5] and _ptr(legal) == rows[6] and
+            (rows[0] <= 1 or (logits.stride(0) == rows[4] and (legal is None or legal.stride(0) == rows[7])))):
+        logits, board, legal, rows = _rows(logits, board, legal)
+        if (rows[0], rows[1], rows[3]) != (ctx.rows[0], ctx.rows[1], ctx.rows[3]) or _on_one_gpu(logits, board, legal) != ctx.device:
+            raise RuntimeError("a saved-tensor hook handed back other logits or masks")
+    for i, (t, was) in enumerate(zip(others, ctx.kept)):
+        if t is not None and (t.data_ptr() != was[0] or not t.is_contiguous()):
+            if t.shape != was[1] or t.dtype != was[2] or t.get_device() != ctx.device:
+                raise RuntimeError(f"a saved-tensor hook handed back {t.dtype} {tuple(t.shape)} on {t.device} for {was[2]} {tuple(was[1])}")
+            others[i] = t.contiguous()
+    return rows, logits, board, legal, *others
 
 
 def _score_forward(logits, moves, board, legal, top, rows, device, keep):
@@ -157,17 +173,15 @@ class _ScoreFunction(torch.autograd.Function):
     def forward(ctx, logits, moves, board, legal, top, rows, device):
         logp, entropy, top_moves, top_logp, stats, bits = _score_forward(logits, moves, board, legal, top, rows, device, True)
         ctx.set_materialize_grads(False)
-        ctx.rows, ctx.device = rows, device
         if top:
             ctx.mark_non_differentiable(top_moves, top_logp)
-        ctx.save_for_backward(logits, moves, board, legal, entropy, stats, bits)
+        _keep(ctx, rows, device, logits, board, legal, moves, entropy, stats, bits)
         return logp, entropy, top_moves, top_logp
 
     @staticmethod
     def backward(ctx, g_logp, g_entropy, _moves, _logp):
         _once()
-        logits, moves, board, legal, entropy, stats, bits = ctx.saved_tensors
-        logits, board, legal, rows = _saved(ctx.rows, logits, board, legal)
+        rows, logits, board, legal, moves, entropy, stats, bits = _kept(ctx)
         if g_logp is None and g_entropy is None:
             return (None,) * 7
         d = logits.new_empty(logits.shape)
@@ -232,8 +246,8 @@ class _LossFunction(torch.autograd.Function):
         d_value = value.new_empty(value.shape) if need_v else None
         _loss_call(rows, device, value, pi, r, None, 0, total, parts, d_logits, d_value)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, value, pi, r, board, legal)
-        ctx.rows, ctx.device, ctx.ready = rows, device, (d_logits, d_value)
+        _keep(ctx, rows, device, logits, board, legal, value, pi, r)
+        ctx.ready = d_logits, d_value
         if want_parts:
             ctx.mark_non_differentiable(parts)
         return total, parts
@@ -241,8 +255,7 @@ class _LossFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g, _parts):
         _once()
-        logits, value, pi, r, board, legal = ctx.saved_tensors
-        logits, board, legal, rows = _saved(ctx.rows, logits, board, legal)
+        rows, logits, board, legal, value, pi, r = _kept(ctx)
         ready, ctx.ready = ctx.ready, None  # given away once: a second backward pass computes its own
         if ready is None:
             need_l, need_v = ctx.needs_input_grad[:2]

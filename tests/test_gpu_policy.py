@@ -555,3 +555,42 @@ def test_more_long_rows_than_a_launch_has_workgroups():
     assert off <= (tS + 3 * (d[mine].abs() + logS.squeeze(1)) * U).sum() + 4 * U * logp[mine].sum().abs()
     del x, pi
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("actions", [225, 1089])
+@pytest.mark.parametrize("mask", ["none", "legal", "board"])
+def test_saved_tensors_laid_out_otherwise_by_a_hook(actions, mask):
+    # a hook may hand back the same numbers with other strides; other types, sizes or devices are refused before a kernel runs
+    from alphazero_amd import policy
+
+    x, legal, pi, v, r = _loss_inputs(30, actions, torch.float32, mask, 4)
+    kw = _mask_args(mask, legal, 1)
+    x = torch.where(legal, x, 0.0).cuda().requires_grad_()
+    pi, v, r = pi.cuda(), v.cuda().requires_grad_(), r.cuda()
+    mv = torch.arange(30, device="cuda")
+
+    def grads(unpack):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            s = policy.score(x, mv, **kw)
+            total = policy.loss(x, v, pi, r, **kw)
+        return [torch.autograd.grad(total, (x, v), torch.tensor(3.0, device="cuda")), torch.autograd.grad((s.entropy, s.logp), x, (r, v.detach()))]
+
+    want = grads(lambda t: t)
+    got = grads(lambda t: torch.stack([t, t], -1)[..., 0])
+    assert all(torch.equal(p, q) for a, b in zip(want, got) for p, q in zip(a, b))
+    for bad in (lambda t: t.cpu(), lambda t: t[:-1].clone(), lambda t: t.double() if t.is_floating_point() else t.short()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, bad):
+            s = policy.score(x, mv, **kw)
+            total = policy.loss(x, v, pi, r, **kw)
+        for f in (total, s.entropy.sum()):
+            with pytest.raises((RuntimeError, ValueError)):
+                torch.autograd.grad(f, x)
+    kept = x.data_ptr()
+    for change in (lambda t: t.double() if t.dtype == torch.float32 and t.data_ptr() != kept else t,  # all but the logits
+                   lambda t: t.cpu() if t.data_ptr() != kept else t):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+            s = policy.score(x, mv, **kw)
+            total = policy.loss(x, v, pi, r, **kw)
+        for f in (total, s.entropy.sum()):
+            with pytest.raises((RuntimeError, ValueError), match="hook|board|GPU of the logits"):
+                torch.autograd.grad(f, x)
