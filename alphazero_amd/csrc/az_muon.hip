@@ -1240,7 +1240,7 @@ int az_muon_orthogonalise(int count, int rows, int cols, const void *const *d_in
     s.ld_in = ld_in;
     s.ld_out = ld_out;
     const bool small = is_small(s);
-    if (!small && !d_work) return AZ_ERR_ARG;
+    if (!small && (!d_work || (uintptr_t)d_work % 16)) return AZ_ERR_ARG;
     const int batch = batch_of(s, count);
     for (int at = 0; at < count;) {
         int n = count - at < batch ? count - at : batch;

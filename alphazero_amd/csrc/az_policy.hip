@@ -960,7 +960,7 @@ int az_policy_score(int n, int actions, const void *d_logits, int dtype, long lo
         });
         return launch_ok();
     }
-    if (!d_work) return AZ_ERR_ARG;
+    if (!d_work || (uintptr_t)d_work % 16) return AZ_ERR_ARG;
     const Chunks c = chunks_of(n, actions, top);
     LongOut w = {};
     w.part = (Part *)d_work;
@@ -1022,7 +1022,7 @@ int az_policy_loss(int n, int actions, const void *d_logits, int dtype, long lon
 {
     const Rows a = {d_logits, ld, d_board, d_legal, ld_legal, n, actions};
     if (!rows_ok(a, dtype) || n < 1) return AZ_ERR_ARG;
-    if (!d_work && (d_loss || actions > SHORT_MAX)) return AZ_ERR_ARG;
+    if ((d_loss || actions > SHORT_MAX) && (!d_work || (uintptr_t)d_work % 16)) return AZ_ERR_ARG;
     if (!d_logits || !d_value || !d_pi || !d_r || (only_if_scaled && !d_scale) || (d_parts && !d_loss)) return AZ_ERR_ARG;
     Loss o = {d_value, value_f32, d_pi, d_r, 1.f / (float)n, d_scale, only_if_scaled, d_loss ? (double *)d_work : nullptr, d_dlogits, d_dvalue};
     const dim3 block(64 * WAVES);

@@ -449,7 +449,8 @@ enum { AZ_POLICY_MAX_MOVES = 64, AZ_POLICY_MAX_TOP = 32 };
  *   d_top_moves, d_top_logp [n][top]   best first, equal logits by lowest index; -1 / -inf where no legal cell above -inf is left;
  *                        NaN cells are never among them
  *   d_stats [n][2], d_mask [n][az_policy_mask_words]   (may be NULL) what az_policy_score_grad needs
- * d_work: az_policy_score_work(n, actions, top) bytes (0 up to 1024 actions), used by this call only. */
+ * d_work: az_policy_score_work(n, actions, top) bytes (0 up to 1024 actions) from a multiple of 16 on, used by this call
+ * only. */
 long long az_policy_score_work(int n, int actions, int top);
 int az_policy_mask_words(int actions);   /* 0: rows this long keep no mask (the gradient reads board / legal again) */
 int az_policy_score(int n, int actions, const void *d_logits, int dtype, long long ld, const float *d_board,
@@ -473,7 +474,8 @@ int az_policy_score_grad(int n, int actions, const void *d_logits, int dtype, lo
  *   d_dlogits [n][actions] (type of the logits), d_dvalue [n] (type of the values): gradients of the total times
  *   *d_scale (device float; NULL: 1); either may be NULL.  only_if_scaled: do nothing when *d_scale is 1 (the buffers
  *   hold the gradients of an earlier call with the same inputs and no scale).
- * d_work: az_policy_loss_work(n, actions) bytes, used by this call only (may be NULL up to 1024 actions when d_loss is). */
+ * d_work: az_policy_loss_work(n, actions) bytes from a multiple of 16 on, used by this call only (may be NULL up to 1024
+ * actions when d_loss is). */
 long long az_policy_loss_work(int n, int actions);
 int az_policy_loss(int n, int actions, const void *d_logits, int dtype, long long ld, const float *d_board,
                    const unsigned char *d_legal, long long ld_legal, const void *d_value, int value_f32, const float *d_pi,
@@ -490,8 +492,8 @@ int az_policy_loss(int n, int actions, const void *d_logits, int dtype, long lon
  * digits (a row of 1e-5 |G| five, of 1e-7 |G| three, of 1e-11 |G| none).  A step multiplies what is missing by up to a; the
  * limit of 10 steps keeps the result as a whole as good as float32 products make it.  The same call gives the same
  * bits (how many matrices there are decides how sums are split, so a matrix alone may differ in the last bits).  d_work:
- * az_muon_work(count, rows, cols) bytes (0 for small matrices), used by this call only; the device current at the call is
- * the one of the pointers and of `stream`. */
+ * az_muon_work(count, rows, cols) bytes (0 for small matrices) from a multiple of 16 on, used by this call only; the device
+ * current at the call is the one of the pointers and of `stream`. */
 enum { AZ_MUON_MAX_DIM = 32768, AZ_MUON_MAX_CELLS = 1 << 28, AZ_MUON_MAX_STEPS = 10 };
 long long az_muon_work(int count, int rows, int cols);
 int az_muon_orthogonalise(int count, int rows, int cols, const void *const *d_in, long long ld_in, void *const *d_out,

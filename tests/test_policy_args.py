@@ -95,3 +95,14 @@ def test_traces_are_refused():
     for f, args in ((policy.score, (X,)), (policy.loss, (X, V, PI, R)), (muon.orthogonalise, (X,))):
         with pytest.raises(RuntimeError, match="cannot be traced"):
             torch.jit.trace(f, args)
+
+
+def test_c_entries_refuse_workspaces_off_their_alignment():
+    import ctypes as C
+
+    L = E.load_library()
+    p, one = 0x1000, (C.c_void_p * 1)(0x1000)  # never looked at
+    for off in (1, 4, 8):
+        assert L.az_policy_score(1, 2000, p, 0, 2000, None, None, 0, None, 4, 0, 1, None, p, p, p, None, None, p + off, None) == E.ERR_ARG
+        assert L.az_policy_loss(1, 9, p, 0, 9, None, None, 0, p, 1, p, p, None, 0, p, None, p, p, p + off, None) == E.ERR_ARG
+        assert L.az_muon_orthogonalise(1, 100, 100, one, 100, one, 100, 0, 5, p + off, None) == E.ERR_ARG
