@@ -522,8 +522,9 @@ template <class T, int R> __global__ __launch_bounds__(64 * WAVES) void k_loss(R
 
 // the total, and the policy and value parts, from the workgroups' partial sums, added in a fixed order
 constexpr int JOIN_WAVES = 16;
-__global__ __launch_bounds__(64 * JOIN_WAVES) void k_loss_join(const double *part, int blocks, double inv_n, float *loss, float *parts)
+__global__ __launch_bounds__(64 * JOIN_WAVES) void k_loss_join(const double *part, int blocks, double inv_n, const float *unless_one, float *loss, float *parts)
 {
+    if (unless_one && *unless_one == 1.f) return; // (nor have the kernels before written partial sums)
     constexpr int EACH = (GRID_MAX + 64 * JOIN_WAVES - 1) / (64 * JOIN_WAVES);
     double2 in[EACH]; // (all in flight together)
 #pragma unroll
@@ -1051,7 +1052,8 @@ int az_policy_loss(int n, int actions, const void *d_logits, int dtype, long lon
             hipLaunchKernelGGL((k_long_loss<T>), dim3(blocks), block, 0, st, a, c, (const Part *)w.part, o);
         });
     }
-    if (d_loss) hipLaunchKernelGGL(k_loss_join, dim3(1), dim3(64 * JOIN_WAVES), 0, st, (const double *)d_work, blocks, 1. / n, d_loss, d_parts);
+    if (d_loss) hipLaunchKernelGGL(k_loss_join, dim3(1), dim3(64 * JOIN_WAVES), 0, st, (const double *)d_work, blocks, 1. / n,
+                                   only_if_scaled ? d_scale : nullptr, d_loss, d_parts);
     return launch_ok();
 }
 

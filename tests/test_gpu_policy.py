@@ -594,3 +594,60 @@ def test_saved_tensors_laid_out_otherwise_by_a_hook(actions, mask):
         for f in (total, s.entropy.sum()):
             with pytest.raises((RuntimeError, ValueError), match="hook|board|GPU of the logits"):
                 torch.autograd.grad(f, x)
+
+
+@pytest.mark.parametrize("actions", [225, 5000])
+def test_c_entry_does_nothing_unless_scaled(actions):
+    # every output stays as it was where the factor is 1, the loss too; with another factor all of them are written
+    from alphazero_amd import engine as E
+
+    L = E.load_library()
+    x, legal, pi, v, r = (t.cuda() for t in _loss_inputs(9, actions, torch.float32, "none", 5))
+    work = torch.empty(L.az_policy_loss_work(9, actions), dtype=torch.uint8, device="cuda").fill_(77)
+
+    def call(scale, only, out):
+        at = torch.tensor(scale, device="cuda")
+        rc = L.az_policy_loss(9, actions, x.data_ptr(), 0, actions, None, None, 0, v.data_ptr(), 1, pi.data_ptr(), r.data_ptr(), at.data_ptr(),
+                              only, *[t.data_ptr() for t in out], work.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        return [t.clone() for t in out]
+
+    fresh = lambda: [torch.full(s, 7.0, device="cuda") for s in ((1,), (2,), (9, actions), (9,))]  # noqa: E731
+    assert all((t == 7).all() for t in call(1.0, 1, fresh()))
+    want = call(3.0, 0, fresh())
+    assert all(torch.equal(a, b) for a, b in zip(call(3.0, 1, fresh()), want))
+    plain = call(1.0, 0, fresh())
+    assert torch.equal(plain[0], want[0]) and torch.equal(plain[1], want[1])  # (the factor is the gradients')
+
+
+@pytest.mark.parametrize("actions,dtype", [(1 << 24, torch.float32), ((1 << 24) - 1, torch.float16)])
+def test_the_longest_rows(actions, dtype):
+    from alphazero_amd import policy
+
+    g = torch.Generator(device="cuda").manual_seed(actions)
+    x = (2 * torch.randn(2, actions, generator=g, device="cuda")).to(dtype)
+    legal = torch.rand(actions, generator=g, device="cuda") < 0.7
+    legal[-1] = True
+    x[0, -1] = 30
+    moves = torch.tensor([[actions - 1, 12345], [actions - 1, 12345]], device="cuda")
+    x.requires_grad_()
+    s = policy.score(x, moves, legal=legal, top=32)
+    at = legal.nonzero().squeeze(1)
+    xd = x.detach()[:, at].double()
+    M = xd.max(1, keepdim=True).values
+    logS = (xd - M).exp().sum(1, keepdim=True).log()
+    p = (xd - M - logS).exp()
+    tS = ((2.5 * (p * (xd - M).abs()).sum(1, keepdim=True) + 16 + actions / 64 / 256) * U).cpu()  # (256 chunks)
+    got = x.detach().gather(1, moves).double()
+    want = torch.where(legal[moves], got - M - logS, -math.inf)
+    _ok(s.logp, want.cpu(), tS + 3 * ((got - M).abs() + logS).cpu() * U, "logp")
+    ranked = xd.sort(dim=1, descending=True, stable=True)
+    assert torch.equal(s.top_moves.long(), at[ranked.indices[:, :32]])
+    H = -(p * (xd - M - logS)).sum(1)
+    assert ((s.entropy - H).abs().cpu() <= 4 * tS.squeeze(1) * (1 + H.cpu())).all()
+    dx, = torch.autograd.grad(s.logp[:, 0].sum(), x)
+    want = torch.zeros_like(x, dtype=torch.float64)
+    want[:, at] = -p
+    want[:, -1] += 1
+    tol = want.abs() * (torch.finfo(dtype).eps / 2 + 200 * U) + 4 * U + (2.0 ** -25 if dtype == torch.float16 else 0)
+    assert ((dx - want).abs() <= tol).all() and not dx[:, ~legal].any()
