@@ -459,3 +459,21 @@ def test_optimiser_goes_on_from_its_saved_state(dtype):
     steps(a, one, grads[3:])
     steps(b, two, grads[3:])
     assert torch.equal(a, b) and two.state[b]["momentum"].data_ptr() != one.state[a]["momentum"].data_ptr()
+
+
+@pytest.mark.parametrize("shape,steps", [((32768, 1), 5), ((1, 32768), 5), ((33, 32768), 5), ((32768, 70), 5), ((16384, 16384), 1), ((8192, 32768), 1)])
+def test_the_largest_sizes(shape, steps):
+    from alphazero_amd import muon
+
+    g = torch.randn(shape, generator=torch.Generator(device="cuda").manual_seed(9), device="cuda")
+    out = muon.orthogonalise(g, steps)
+    x = g.double()  # (the definition on the GPU, in 64 bits)
+    x = x.t().contiguous() if shape[0] > shape[1] else x
+    x = x / x.square().sum().sqrt()
+    for _ in range(steps):
+        A = x @ x.t().contiguous()
+        x = ABC[0] * x + (ABC[1] * A + ABC[2] * (A @ A)) @ x
+    x = x.t() if shape[0] > shape[1] else x
+    size = x.norm()
+    assert (out.double() - x).norm() <= ABC[0] ** (steps - 1) * 1.41 * 32 * U + size * 64 * U
+    torch.cuda.empty_cache()
