@@ -20,6 +20,14 @@ class _Scores:
         entropy and the `top` best alternatives of the network's policy over the legal moves of each position."""
         from . import policy
 
+        # (checked here: the fused kernel takes an address, and a search hands it the engine's own boards)
+        size = getattr(self, "shape", None)
+        if not torch.is_tensor(boards) or boards.dtype != torch.float32 or boards.dim() != 4 or boards.shape[1] != 2 \
+                or boards.shape[2] != boards.shape[3] or size not in (None, boards.shape[2]):
+            side = "S" if size is None else size
+            raise ValueError(f"boards must be float32 [n, 2, {side}, {side}]")
+        if not boards.is_cuda or boards.device.index != (0 if self.device.index is None else self.device.index):
+            raise ValueError("boards must be on the evaluator's GPU (there is no CPU path)")
         value, logp = self(boards)
         return value, policy.score(logp, moves, board=boards, top=top)
 
@@ -38,7 +46,7 @@ class TorchEvaluator(_Scores):
     def __call__(self, boards):
         value, logp = self.module(boards)
         return (value.reshape(-1).to(torch.float32).contiguous(),
-                logp.reshape(boards.shape[0], -1).to(torch.float32).contiguous())
+                logp.reshape(boards.shape[0], -1 if logp.numel() else boards.shape[-1] ** 2).to(torch.float32).contiguous())
 
 
 class TorchScriptEvaluator(TorchEvaluator):

@@ -651,3 +651,20 @@ def test_the_longest_rows(actions, dtype):
     want[:, -1] += 1
     tol = want.abs() * (torch.finfo(dtype).eps / 2 + 200 * U) + 4 * U + (2.0 ** -25 if dtype == torch.float16 else 0)
     assert ((dx - want).abs() <= tol).all() and not dx[:, ~legal].any()
+
+
+def test_evaluators_score_batches_of_none_and_strided_boards():
+    from alphazero_amd.evaluator import FusedNetEvaluator, TorchEvaluator
+    from alphazero_amd.model import PolicyValueNet
+
+    torch.manual_seed(0)
+    net = PolicyValueNet(9).eval()
+    wide = torch.zeros(5, 2, 9, 12, device="cuda")
+    wide[2, 1, 4, 5] = wide[3, 0, 0, 0] = 1
+    boards, mv = wide[..., :9], torch.arange(5, device="cuda")
+    for ev in (FusedNetEvaluator(net, 9), TorchEvaluator(net), TorchEvaluator(net, torch.device("cuda"))):
+        value, s = ev.score(boards, mv, top=3)
+        v2, want = ev.score(boards.contiguous(), mv, top=3)
+        assert (value - v2).abs().max() < 1e-5 and (s.logp - want.logp).abs().max() < 1e-4
+        value, s = ev.score(boards[:0].contiguous(), mv[:0], top=2)
+        assert value.shape == (0,) and s.logp.shape == (0,) and s.top_moves.shape == (0, 2)

@@ -106,3 +106,20 @@ def test_c_entries_refuse_workspaces_off_their_alignment():
         assert L.az_policy_score(1, 2000, p, 0, 2000, None, None, 0, None, 4, 0, 1, None, p, p, p, None, None, p + off, None) == E.ERR_ARG
         assert L.az_policy_loss(1, 9, p, 0, 9, None, None, 0, p, 1, p, p, None, 0, p, None, p, p, p + off, None) == E.ERR_ARG
         assert L.az_muon_orthogonalise(1, 100, 100, one, 100, one, 100, 0, 5, p + off, None) == E.ERR_ARG
+
+
+def test_evaluators_refuse_boards_they_are_not_made_for():
+    # the fused kernel reads n boards of its own size at an address on the GPU, whatever stands there
+    from alphazero_amd.evaluator import FusedNetEvaluator, TorchEvaluator
+    from alphazero_amd.model import PolicyValueNet
+
+    net = PolicyValueNet(7).eval()
+    good = torch.zeros(3, 2, 7, 7)
+    for ev in (FusedNetEvaluator(net, 7, torch.device("cpu")), TorchEvaluator(net, torch.device("cpu"))):
+        for bad in (good.double(), good.to(torch.uint8), good[:, :1], good[0], good[:, :, :6], good.tolist()):
+            with pytest.raises(ValueError, match="boards must be float32"):
+                ev.score(bad)
+        with pytest.raises(ValueError, match="no CPU path"):
+            ev.score(good)
+    with pytest.raises(ValueError, match=r"\[n, 2, 7, 7\]"):
+        FusedNetEvaluator(net, 7, torch.device("cpu")).score(torch.zeros(3, 2, 6, 6))
