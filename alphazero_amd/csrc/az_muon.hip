@@ -1009,12 +1009,16 @@ void gemm(Gemm a, int M, int N, bool turn, int batch, int dtype, const Ptrs &p, 
             a.split = most;
             whole = 0;
         }
-    } else if (big && groups > CUS && groups < 4 * CUS && a.K >= 2048) {
+    } else if (big && groups > CUS && groups < 4 * CUS) {
         // A few large tiles more than CUs: a CU that gets another one doubles its time, so the last ones are shared by as
         // many workgroups as there are CUs.  272 tiles, K = 4096 / 2048: 151 / 85 us -> 116 + 9 / 67 + 10 us (with the
-        // joining); 288 tiles, K = 1024: 46 -> 43 + 7 us, so not there.
+        // joining); 288 tiles, K = 1024: 46 -> 43 + 7 us, so not there.  The more tiles are left, the fewer share each and the
+        // more there is to join, and a short K saves less.  Five steps of one matrix, shared / not, with 256 + `rest` tiles:
+        // K = 1024, rest 8: 478 / 479 us;  K = 1280, rest 4: 506 / 516, 14: 497 / 503, 24: 509 / 503, 64: 541 / 529;  K = 1536,
+        // rest 8: 652 / 677, 44: 673 / 677, 68: 702 / 700, 116: 767 / 740;  K = 2048, rest 16: 880 / 896, 64: 932 / 943, 80: 959 /
+        // 962, 96: 987 / 977, 112: 1013 / 995;  K = 3200, rest 113 and 69: 2272 / 2385.
         const long long rest = groups % CUS;
-        if (rest && rest <= CUS / 2) {
+        if (rest && rest <= CUS / 2 && 12 * rest <= a.K - 1024) {
             ks = 2;
             a.split = (int)(CUS / rest);
             if (a.split > a.K / BK / 4) a.split = a.K / BK / 4;

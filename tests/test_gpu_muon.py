@@ -477,3 +477,23 @@ def test_the_largest_sizes(shape, steps):
     size = x.norm()
     assert (out.double() - x).norm() <= ABC[0] ** (steps - 1) * 1.41 * 32 * U + size * 64 * U
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("shape", [(1280, 3328), (1300, 3400), (1536, 2816), (2432, 1792), (1150, 3700), (1280, 3968)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_last_tiles_shared_from_a_smaller_k_on(shape, dtype):
+    # 260 to 310 large tiles for 256 CUs, on both sides of the rule
+    from alphazero_amd import muon
+
+    g = _updates(shape, 61).to(dtype).cuda()
+    out = muon.orthogonalise(g, 3)
+    assert torch.equal(out, muon.orthogonalise(g, 3))
+    x = g.double()  # (the definition on the GPU, in 64 bits)
+    x = x.t().contiguous() if shape[0] > shape[1] else x
+    x = x / x.square().sum().sqrt()
+    for _ in range(3):
+        A = x @ x.t().contiguous()
+        x = ABC[0] * x + (ABC[1] * A + ABC[2] * (A @ A)) @ x
+    x = x.t() if shape[0] > shape[1] else x
+    size = x.norm()
+    assert (out.double() - x).norm() <= ABC[0] ** 2 * 1.41 * 32 * U + size * (64 * U + (torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0))
