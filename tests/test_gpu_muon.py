@@ -497,3 +497,41 @@ def test_last_tiles_shared_from_a_smaller_k_on(shape, dtype):
     x = x.t() if shape[0] > shape[1] else x
     size = x.norm()
     assert (out.double() - x).norm() <= ABC[0] ** 2 * 1.41 * 32 * U + size * (64 * U + (torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0))
+
+
+def test_a_captured_step():
+    # forward pass, backward pass and update of weights of both kinds in one graph, between eager steps of a twin
+    from alphazero_amd import muon
+
+    torch.manual_seed(5)
+    shapes = [(24, 30), (100, 140)]
+    x = torch.ones((), device="cuda")
+
+    def program():
+        gen = torch.Generator().manual_seed(54)
+        w = [torch.nn.Parameter((torch.randn(*s, generator=gen) * 0.1).to(t).cuda()) for s in shapes for t in (torch.float32, torch.bfloat16)]
+        opt = muon.Muon(w, lr=0.05, weight_decay=0.01)
+
+        ones = [torch.ones(p.shape, device="cuda") for p in w]
+
+        def step():
+            for p, g in zip(w, torch.autograd.grad([torch.tanh(p.float() * x) for p in w], w, ones)):
+                p.grad.copy_(g)
+            opt.step()
+
+        for p in w:
+            p.grad = torch.zeros_like(p)
+        return w, step
+
+    (a, eager), (b, captured) = program(), program()
+    eager(), captured()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured()
+    for k in range(4):
+        x.add_(0.1 * k)
+        eager()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(a, b)), k

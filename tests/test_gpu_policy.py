@@ -668,3 +668,28 @@ def test_evaluators_score_batches_of_none_and_strided_boards():
         assert (value - v2).abs().max() < 1e-5 and (s.logp - want.logp).abs().max() < 1e-4
         value, s = ev.score(boards[:0].contiguous(), mv[:0], top=2)
         assert value.shape == (0,) and s.logp.shape == (0,) and s.top_moves.shape == (0, 2)
+
+
+def test_under_checkpointing_and_inference_mode():
+    from torch.utils.checkpoint import checkpoint
+
+    from alphazero_amd import policy
+
+    x, legal, pi, v, r = (t.cuda() for t in _loss_inputs(30, 225, torch.float32, "legal", 8))
+    x = torch.where(legal, x, 0.0)
+    w = (torch.eye(225, device="cuda") * 2).requires_grad_()
+    mv = torch.arange(30, device="cuda")
+
+    def f(w):
+        rows = x @ w
+        s = policy.score(rows, mv, legal=legal, top=2)
+        return policy.loss(rows, v, pi, r, legal=legal) * 3 + s.entropy.sum()
+
+    want, = torch.autograd.grad(f(w), w)
+    for reentrant in (False, True):
+        w.grad = None
+        checkpoint(f, w, use_reentrant=reentrant).backward()
+        assert torch.equal(w.grad, want)
+    with torch.inference_mode():
+        total = f(w)
+    assert torch.equal(total, f(w).detach()) and not total.requires_grad
