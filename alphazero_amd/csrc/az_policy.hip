@@ -559,7 +559,7 @@ struct LongOut {
     float *list_v;          // [n][chunks][top]
     int *list_i;
     int top;
-    const float *pi;        // or NULL
+    const float *pi;        // of the loss
     const float *unless_one; // device scalar: nothing to do when it is 1; or NULL
 };
 
@@ -572,7 +572,7 @@ __device__ __forceinline__ void rebase(float &S, float &U, float from, float to)
     S = s;
 }
 
-template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_parts(Rows a, Chunks c, LongOut o, long long first)
+template <class T, bool LOSS> __global__ __launch_bounds__(64 * WAVES) void k_long_parts(Rows a, Chunks c, LongOut o, long long first)
 {
     if (o.unless_one && *o.unless_one == 1.f) return;
     const int lane = threadIdx.x & 63;
@@ -582,7 +582,7 @@ template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_parts(Ro
     const int chunk = (int)(unit - row * c.count);
     const int begin = chunk * c.len, end = min(a.A, begin + c.len);
     const T *p = (const T *)a.x + (size_t)row * a.ld;
-    const float *pi = o.pi ? o.pi + (size_t)row * a.A : nullptr;
+    const float *pi = LOSS ? o.pi + (size_t)row * a.A : nullptr;
     float M = NINF, S = 0.f, U = 0.f, W = 0.f, E = 0.f, X = 0.f; // S, U, W, E, X: this lane's share; M: the wavefront's
     Best best = {NINF, -1};
     for (int j0 = begin; j0 < end; j0 += LONG_STEP) {
@@ -590,7 +590,7 @@ template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_parts(Ro
         bool ok[LONG_R];
 #pragma unroll
         for (int r = 0; r < LONG_R; r++) x[r] = get(p, min(j0 + r * 64 + lane, end - 1));
-        if (pi) {
+        if (LOSS) {
 #pragma unroll
             for (int r = 0; r < LONG_R; r++) q[r] = pi[min(j0 + r * 64 + lane, end - 1)];
         }
@@ -606,7 +606,7 @@ template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_parts(Ro
         m = wave_max(m);
         if (m > M) {
             if (M != NINF) {
-                if (pi) X += W == 0.f ? 0.f : W * (M - m);
+                if (LOSS) X += W == 0.f ? 0.f : W * (M - m);
                 rebase(S, U, M, m);
             }
             M = m;
@@ -617,18 +617,18 @@ template <class T> __global__ __launch_bounds__(64 * WAVES) void k_long_parts(Ro
             const float e = x[r] == NINF ? 0.f : exp_neg(d);
             S += e;
             U += e == 0.f ? 0.f : e * d;
-            if (pi) {
+            if (LOSS) {
                 const float w = ok[r] ? q[r] : 0.f;
                 W += w;
                 E += w * log_of(w);
                 X += w == 0.f ? 0.f : w * (x[r] == NINF ? NINF : d); // (M is -inf until a cell above it comes)
             }
         }
-        if (o.top) best_offer<LONG_R>(best, x, j0, o.top, lane);
+        if (!LOSS && o.top) best_offer<LONG_R>(best, x, j0, o.top, lane);
     }
     Part out = {M, wave_sum(S), wave_sum(U), wave_sum(W), wave_sum(E), wave_sum(X)};
     if (lane == 0) o.part[unit] = out;
-    if (o.top && lane < o.top) {
+    if (!LOSS && lane < o.top) {
         o.list_v[(size_t)unit * o.top + lane] = best.v;
         o.list_i[(size_t)unit * o.top + lane] = best.i;
     }
@@ -971,7 +971,7 @@ int az_policy_score(int n, int actions, const void *d_logits, int dtype, long lo
     by_type(dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
         in_launches(groups_of(n, c), [&](long long first, dim3 grid) {
-            hipLaunchKernelGGL((k_long_parts<T>), grid, block, 0, st, a, c, w, first);
+            hipLaunchKernelGGL((k_long_parts<T, false>), grid, block, 0, st, a, c, w, first);
         });
         in_launches(n, [&](long long first, dim3 grid) {
             hipLaunchKernelGGL((k_long_score<T>), grid, block, (size_t)c.count * top * 8, st, a, c, w, o, first);
@@ -1047,7 +1047,7 @@ int az_policy_loss(int n, int actions, const void *d_logits, int dtype, long lon
         by_type(dtype, [&](auto *t) {
             using T = std::remove_pointer_t<decltype(t)>;
             in_launches(groups_of(n, c), [&](long long first, dim3 grid) {
-                hipLaunchKernelGGL((k_long_parts<T>), grid, block, 0, st, a, c, w, first);
+                hipLaunchKernelGGL((k_long_parts<T, true>), grid, block, 0, st, a, c, w, first);
             });
             hipLaunchKernelGGL((k_long_loss<T>), dim3(blocks), block, 0, st, a, c, (const Part *)w.part, o);
         });
