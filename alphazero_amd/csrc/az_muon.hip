@@ -1,6 +1,7 @@
 // Newton-Schulz orthogonalisation of weight updates (gfx950): the singular values of G / |G|_F go through
 //   p(s) = a s + b s^3 + c s^5,   (a, b, c) = (3.4445, -4.7750, 2.0315),
-// `steps` times, which moves all but the smallest near 1 and leaves the singular vectors alone.
+// `steps` times, which moves all but the smallest near 1 and leaves the singular vectors alone (the coefficients: K. Jordan et
+// al., "Muon: An optimizer for hidden layers in neural networks", 2024).
 //
 // With m <= n (a taller matrix is taken transposed), A = X X' and Q = a I + b A + c A^2, one step is X <- Q X and makes
 // the next Gram matrix A' = Q A Q = Q^2 A: all m x m factors are polynomials of one symmetric matrix, they commute and

@@ -1,5 +1,6 @@
 """Orthogonalised weight updates on the GPU: `orthogonalise` (Newton-Schulz steps on matrices of updates) and `Muon`, the
-optimiser that applies them to a network's weight matrices.
+optimiser that applies them to a network's weight matrices (K. Jordan et al., "Muon: An optimizer for hidden layers in neural
+networks", 2024: the coefficients, the momentum and the factor for weights with more rows than columns).
 
 The HIP kernels (csrc/az_muon.hip, reached through the C ABI) run on torch's current stream of the tensors' device; they
 allocate through torch, wait for nothing and can be captured into a graph."""

@@ -492,8 +492,8 @@ int az_policy_loss(int n, int actions, const void *d_logits, int dtype, long lon
  * digits (a row of 1e-5 |G| five, of 1e-7 |G| three, of 1e-11 |G| none).  A step multiplies what is missing by up to a; the
  * limit of 10 steps keeps the result as a whole as good as float32 products make it.  The same call gives the same
  * bits (how many matrices there are decides how sums are split, so a matrix alone may differ in the last bits).  d_work:
- * az_muon_work(count, rows, cols) bytes (0 for small matrices) from a multiple of 16 on, used by this call only; the device
- * current at the call is the one of the pointers and of `stream`. */
+ * az_muon_work(count, rows, cols) bytes (0 for small matrices; at most 1 GiB, or what one matrix takes) from a multiple
+ * of 16 on, used by this call only; the device current at the call is the one of the pointers and of `stream`. */
 enum { AZ_MUON_MAX_DIM = 32768, AZ_MUON_MAX_CELLS = 1 << 28, AZ_MUON_MAX_STEPS = 10 };
 long long az_muon_work(int count, int rows, int cols);
 int az_muon_orthogonalise(int count, int rows, int cols, const void *const *d_in, long long ld_in, void *const *d_out,
