@@ -277,8 +277,8 @@ def loss(logits, value, pi, r, *, board=None, legal=None, parts=False):
     pi      float32 [n, actions], targets (rows need not sum to 1; masked cells are not looked at, a target on a legal cell
             at -inf makes the loss infinite);  r  float32, n results
 
-    Differentiable (once, in reverse mode) for logits and value.  parts=True returns (total, policy part, value part), the parts without
-    gradient.  Zero records give 0."""
+    Differentiable (once, in reverse mode) for logits and value.  parts=True returns (total, policy part, value part), the
+    parts without gradient.  Zero records give 0."""
     _untraced("policy.loss")
     if _forward._current_level >= 0:
         _without_tangents(logits, value, pi, r)
